@@ -7,7 +7,9 @@
 
 typedef __bf16 rl_bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 rl_f16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t rl_u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t rl_u32x4 __attribute__((ext_vector_type(4)));
+typedef float rl_f32x2 __attribute__((ext_vector_type(2)));
 typedef float rl_f32x4 __attribute__((ext_vector_type(4)));
 
 #define RL_LDS __attribute__((address_space(3)))

@@ -34,6 +34,11 @@ class KvLayoutDesc(C.Structure):
         row = head_dim * scalar_bytes
         return cls(token_count, head_dim, scalar_bytes, 16, row, row, 2 * token_count * row, 128)
 
+    @classmethod
+    def paged8(cls, token_count: int, head_dim: int) -> "KvLayoutDesc":
+        """e4m3 blocks with their planes' scales behind them (kv_layout_desc_paged8)."""
+        return cls(token_count, head_dim, 1, 16, head_dim, head_dim, 2 * token_count * head_dim + 128, 128)
+
 
 class HwDesc(C.Structure):
     _pack_ = 1
@@ -227,6 +232,24 @@ class AppendArgs(C.Structure):
                 ("k_new", C.c_void_p), ("v_new", C.c_void_p)]
 
 
+class AttnPromptArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p),
+                ("q_stride", C.c_uint32), ("k_stride", C.c_uint32), ("v_stride", C.c_uint32),
+                ("out_stride", C.c_uint32), ("q_starts", C.c_void_p), ("kv_starts", C.c_void_p),
+                ("seqs", C.c_uint32), ("q_tokens", C.c_uint32), ("kv_tokens", C.c_uint32), ("max_q", C.c_uint32),
+                ("max_kv", C.c_uint32), ("q_heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("dtype", C.c_uint32), ("scale", C.c_float), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
+class Kv8AppendArgs(C.Structure):
+    _fields_ = [("arena_base", C.c_void_p), ("arena_bytes", C.c_uint64), ("layout", KvLayoutDesc),
+                ("block_table", C.c_void_p), ("table_stride", C.c_uint32), ("batch", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("dtype", C.c_uint32), ("positions", C.c_void_p), ("starts", C.c_void_p),
+                ("tokens", C.c_uint32), ("max_new", C.c_uint32), ("cow_src", C.c_void_p), ("k_new", C.c_void_p),
+                ("v_new", C.c_void_p), ("k_stride", C.c_uint32), ("v_stride", C.c_uint32)]
+
+
 class ProjArgs(C.Structure):
     _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("logits", C.c_void_p), ("rows", C.c_uint32),
                 ("vocab", C.c_uint32), ("hidden", C.c_uint32), ("x_stride", C.c_uint32),
@@ -338,6 +361,11 @@ def load(path: str = LIB_PATH) -> C.CDLL:
                                            C.POINTER(AppendArgs), C.c_void_p, C.c_void_p, C.c_size_t]),
         "rl_hip_decode_lane_flush": (i32, [i32, C.POINTER(AttnArgs), C.POINTER(AppendArgs), C.c_void_p,
                                             C.c_size_t]),
+        "rl_hip_attn_prompt_workspace": (sz, [C.POINTER(AttnPromptArgs)]),
+        "rl_hip_attn_prompt": (i32, [C.POINTER(AttnPromptArgs)]),
+        "rl_hip_kv8_append": (i32, [C.POINTER(Kv8AppendArgs)]),
+        "rl_hip_attn_decode_kv8_workspace": (sz, [C.POINTER(AttnArgs)]),
+        "rl_hip_attn_decode_kv8": (i32, [C.POINTER(AttnArgs)]),
         "rl_hip_logits_proj": (i32, [C.POINTER(ProjArgs)]),
         "rl_hip_reward_advantage": (i32, [C.POINTER(RewardArgs)]),
         "rl_hip_rollout_schedule": (i32, [C.POINTER(SchedArgs)]),
@@ -675,6 +703,47 @@ def sample_workspace(args: SampleArgs) -> DeviceBuffer:
 
 def sample(args: SampleArgs) -> None:
     check(lib().rl_hip_sample(C.byref(args)), "rl_hip_sample")
+
+
+def attn_prompt_workspace_bytes(args: AttnPromptArgs) -> int:
+    n = lib().rl_hip_attn_prompt_workspace(C.byref(args))
+    if n == 0:
+        raise RlrtError(f"rl_hip_attn_prompt_workspace: {_err()}")
+    return int(n)
+
+
+def attn_prompt_workspace(args: AttnPromptArgs) -> DeviceBuffer:
+    ws = DeviceBuffer(attn_prompt_workspace_bytes(args))
+    args.workspace, args.workspace_bytes = ws.ptr, ws.nbytes
+    return ws
+
+
+def attn_prompt(args: AttnPromptArgs) -> None:
+    """Causal attention over packed whole prompts."""
+    check(lib().rl_hip_attn_prompt(C.byref(args)), "rl_hip_attn_prompt")
+
+
+def kv8_append(args: Kv8AppendArgs) -> None:
+    """K/V rows (prompts, or one token per row) into an 8-bit arena."""
+    check(lib().rl_hip_kv8_append(C.byref(args)), "rl_hip_kv8_append")
+
+
+def attn_kv8_workspace_bytes(args: AttnArgs) -> int:
+    n = lib().rl_hip_attn_decode_kv8_workspace(C.byref(args))
+    if n == 0:
+        raise RlrtError(f"rl_hip_attn_decode_kv8_workspace: {_err()}")
+    return int(n)
+
+
+def attn_kv8_workspace(args: AttnArgs) -> DeviceBuffer:
+    ws = DeviceBuffer(attn_kv8_workspace_bytes(args))
+    args.workspace, args.workspace_bytes = ws.ptr, ws.nbytes
+    return ws
+
+
+def attn_decode_kv8(args: AttnArgs) -> None:
+    """attn_decode over an 8-bit arena (layout KvLayoutDesc.paged8)."""
+    check(lib().rl_hip_attn_decode_kv8(C.byref(args)), "rl_hip_attn_decode_kv8")
 
 
 def kv_append(args: AppendArgs) -> None:

@@ -115,3 +115,43 @@ kv_layout_check_paged(const KvLayoutDesc *d)
         return -1;
     return 0;
 }
+
+/* ---- 8-bit blocks ----------------------------------------------------------
+ * A block of the 8-bit cache holds `token_count` tokens of one KV head as
+ * e4m3 bytes (1 sign, 4 exponent and 3 mantissa bits, largest value 448): the
+ * K plane, the V plane, then the planes' two fp32 scales (K, V; a byte stands
+ * for its e4m3 value times its plane's scale, a power of two) and padding to
+ * the alignment. No reference counterpart (its blocks are 2-byte scalars). */
+#define KV_LAYOUT8_TAIL_BYTES KV_LAYOUT_ALIGNMENT
+
+static inline KvLayoutDesc
+kv_layout_desc_paged8(uint32_t token_count, uint32_t head_dim)
+{
+    KvLayoutDesc d = kv_layout_desc_paged(token_count, head_dim, 1u);
+    d.block_bytes += KV_LAYOUT8_TAIL_BYTES;
+    return d;
+}
+
+static inline uint32_t
+kv_layout8_scale_offset_bytes(const KvLayoutDesc *d)
+{
+    return 2u * d->token_count * d->head_dim;
+}
+
+/* 0 when the layout is one the 8-bit kernels accept (kv_layout_desc_paged8 of
+ * 16 or 32 tokens and head_dim 64 or 128), -1 otherwise. */
+static inline int
+kv_layout_check_paged8(const KvLayoutDesc *d)
+{
+    if (!d)
+        return -1;
+    if (d->token_count != 16u && d->token_count != 32u)
+        return -1;
+    if (d->head_dim != 64u && d->head_dim != 128u)
+        return -1;
+    if (d->scalar_bytes != 1u || d->k_stride_bytes != d->head_dim || d->v_stride_bytes != d->head_dim)
+        return -1;
+    if (d->block_bytes != kv_layout8_scale_offset_bytes(d) + KV_LAYOUT8_TAIL_BYTES)
+        return -1;
+    return 0;
+}

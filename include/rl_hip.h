@@ -126,6 +126,100 @@ typedef struct {
 size_t rl_hip_attn_decode_workspace(const rl_attn_decode_args_t *args);
 int rl_hip_attn_decode(const rl_attn_decode_args_t *args);
 
+/* ---- attention over whole prompts -------------------------------------------
+ * No reference function (its worker decodes single tokens over a cache that
+ * is already there). Causal attention of packed sequences: sequence s has the
+ * queries q_starts[s] .. q_starts[s + 1] - 1 and the keys and values
+ * kv_starts[s] .. kv_starts[s + 1] - 1 (kv_starts NULL: the same rows). The
+ * queries are the sequence's last tokens: query i of Lq sees the keys j <= i +
+ * Lk - Lq, so a prompt may be fed in pieces. Query head h reads KV head h /
+ * (q_heads / kv_heads). out = softmax(scale q K^T) V with fp32 sums, the
+ * weights rounded to the inputs' type, stored in it. A query that sees no key
+ * (Lk < Lq) yields zeros. What a query does not see has no part in its output,
+ * NaN and infinities included. Rows of out that belong to no sequence are left
+ * as they were; rows of q, k and v past q_tokens and kv_tokens are never read.
+ * out may not overlap the inputs. */
+typedef struct {
+    const void *q;               /* device [q_tokens][q_heads][head_dim], tokens q_stride elements apart */
+    const void *k;               /* device [kv_tokens][kv_heads][head_dim], k_stride apart */
+    const void *v;               /* device [kv_tokens][kv_heads][head_dim], v_stride apart */
+    void *out;                   /* device [q_tokens][q_heads][head_dim], out_stride apart */
+    uint32_t q_stride;           /* elements; 0: tokens follow each other without a gap. Else a multiple */
+    uint32_t k_stride;           /* of 8, at least a token's own elements, at most 2^24 */
+    uint32_t v_stride;
+    uint32_t out_stride;
+    const uint32_t *q_starts;    /* device [seqs + 1], not decreasing */
+    const uint32_t *kv_starts;   /* device [seqs + 1] or NULL: q_starts */
+    uint32_t seqs;               /* 1 .. 65,535 */
+    uint32_t q_tokens;           /* rows of q and out */
+    uint32_t kv_tokens;          /* rows of k and v */
+    uint32_t max_q;              /* upper bound of the sequences' queries; later ones get no output */
+    uint32_t max_kv;             /* upper bound of their keys (it only guides the split of the work) */
+    uint32_t q_heads;
+    uint32_t kv_heads;           /* divides q_heads */
+    uint32_t head_dim;           /* 64 or 128 */
+    uint32_t dtype;              /* RL_DTYPE_* of q, k, v and out */
+    float scale;                 /* positive; 0 selects 1/sqrt(head_dim) */
+    void *workspace;             /* device, >= rl_hip_attn_prompt_workspace() */
+    size_t workspace_bytes;
+} rl_attn_prompt_args_t;
+
+size_t rl_hip_attn_prompt_workspace(const rl_attn_prompt_args_t *args);
+int rl_hip_attn_prompt(const rl_attn_prompt_args_t *args);
+
+/* ---- the 8-bit KV cache -------------------------------------------------------
+ * No reference function (its cache is 2-byte scalars). An arena whose layout
+ * is kv_layout_desc_paged8: e4m3 blocks, each plane (K, V) with one
+ * power-of-two fp32 scale behind the planes. Half the bytes of the 16-bit
+ * arena, so half the time of a decode step that streams it.
+ *
+ * rl_hip_kv8_append writes row b's new tokens at positions[b], positions[b] +
+ * 1, ...: the rows starts[b] .. starts[b + 1] - 1 of k_new and v_new (at most
+ * max_new), or row b alone when starts is NULL. In every block they reach, a
+ * plane's scale s becomes the smallest power of two with 448 s >= the
+ * magnitude of each finite new value (2^-126 at least), or stays if the block
+ * holds earlier tokens of the row (slots below positions[b]) at a larger one;
+ * new values x become e4m3(x / s), NaN and infinities NaN, and earlier values
+ * are brought to s where it grew: only their exponents move, but for values
+ * that end below 2^-6 s, which are rounded again. With cow_src[b * kv_heads +
+ * g] >= 0 the earlier slots of row b's first block are taken from that
+ * (shared) block of the arena instead, as in rl_hip_kv_append. Slots behind
+ * the last new token keep their bytes and mean nothing. Positions past the
+ * block table and blocks past arena_bytes are skipped. Two rows of one call
+ * must not write the same block.
+ *
+ * rl_hip_attn_decode_kv8 is rl_hip_attn_decode over such an arena, with its
+ * arguments and rules: one query token per row, zeros for a context of 0, NaN
+ * for a row whose context exceeds max_ctx or whose table names a block past
+ * arena_bytes. The products are those of the e4m3 values times their scales
+ * with fp32 sums (within 1e-4 of fp64). Any q_heads / kv_heads from 1 to 16;
+ * grid_waves must be 0. A row's result depends on its own inputs and on
+ * batch, kv_heads and max_ctx, not on the other rows. */
+typedef struct {
+    void *arena_base;            /* device, 16-byte aligned */
+    uint64_t arena_bytes;        /* blocks past it are never read or written */
+    KvLayoutDesc layout;         /* must pass kv_layout_check_paged8 */
+    const uint32_t *block_table; /* device [batch][kv_heads][table_stride] */
+    uint32_t table_stride;
+    uint32_t batch;
+    uint32_t kv_heads;
+    uint32_t dtype;              /* RL_DTYPE_* of k_new and v_new */
+    const uint32_t *positions;   /* device [batch]: of each row's first new token */
+    const uint32_t *starts;      /* device [batch + 1], not decreasing, or NULL: one token per row */
+    uint32_t tokens;             /* rows of k_new and v_new (batch without starts); never read past */
+    uint32_t max_new;            /* upper bound of a row's new tokens; 1 without starts */
+    const int32_t *cow_src;      /* device [batch][kv_heads] or NULL */
+    const void *k_new;           /* device [tokens][kv_heads][head_dim], 16-byte aligned */
+    const void *v_new;
+    uint32_t k_stride;           /* elements between tokens: 0 (no gap) or a multiple of 8 */
+    uint32_t v_stride;
+} rl_kv8_append_args_t;
+
+int rl_hip_kv8_append(const rl_kv8_append_args_t *args);
+
+size_t rl_hip_attn_decode_kv8_workspace(const rl_attn_decode_args_t *args);
+int rl_hip_attn_decode_kv8(const rl_attn_decode_args_t *args);
+
 /* ---- logits projection ------------------------------------------------------
  * No reference function (the nearest analog is the fp16 GEMV
  * query_prepare_kernel, cu/query_producer.cu:5-26). logits[r][v] =

@@ -1,0 +1,241 @@
+"""rl_hip_attn_prompt against attention in 64 bits, and a prompt taken through
+the whole path: prompt attention, the 8-bit cache, decode steps."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import kv8_helpers as k8
+
+pytestmark = pytest.mark.gpu
+
+
+def tolerance(dtype, ref, mag, q, k, scale, n):
+    """What rounding may do to an output o = sum w_j v_j / sum w_j of n keys. The weights are rounded to 16 bits (half a
+    step u each; fp16 weights below 2^-14 by at most 2^-25, relative to a largest weight of 1 or more) and the output
+    once more (u |o|): u (mag + |o|), mag = sum w_j |v_j| / sum w_j. A score is a sum of head_dim fp32 products, off by
+    at most (head_dim + 2) 2^-24 scale sum |q k|, which moves a weight and the sum of weights by that much relatively
+    (2 x mag); exp2, the fp32 sums over n keys and the division add less than (n + 16) 2^-24 mag."""
+    u = k8.HALF_STEP[dtype]
+    d = q.shape[-1]
+    score = (d + 2) * 2.0 ** -24 * scale * np.abs(q).sum(-1).max() * np.abs(k).max()
+    small = n * 2.0 ** -25 if dtype == "fp16" else 0.0
+    return u * (mag + np.abs(ref)) * 1.01 + (2 * score + (n + 16) * 2.0 ** -24) * mag + small * mag.max(initial=0) + 1e-30
+
+
+def compare(got, q, k, v, q_starts, kv_starts, kvh, dtype, scale=None, rows=None):
+    """got, q [tokens][heads][d], k, v [tokens][kv heads][d] as 16-bit arrays."""
+    f = [k8.floats(x, dtype) for x in (got, q, k, v)]
+    group, d = q.shape[1] // kvh, q.shape[2]
+    scale = scale or d ** -0.5
+    for s in range(len(q_starts) - 1):
+        a, b, c, e = q_starts[s], q_starts[s + 1], kv_starts[s], kv_starts[s + 1]
+        seen = [i + 1 + (e - c) - (b - a) for i in range(b - a)]
+        for h in range(q.shape[1]):
+            kk, vv = f[2][c:e, h // group], f[3][c:e, h // group]
+            ref, mag = k8.attend(f[1][a:b, h], kk, vv, scale, seen)
+            if b > a:
+                tol = tolerance(dtype, ref, mag, f[1][a:b, h], kk if e > c else np.zeros((1, d)), scale, e - c)
+                off = np.abs(f[0][a:b, h] - ref)
+                assert (off <= tol).all(), (s, h, float(np.nanmax(off / tol)), np.argwhere(~(off <= tol))[:4].tolist())
+
+
+def inputs(rng, nq, nk, qh, kvh, d, dtype, q_size=1.0):
+    return (k8.bits(rng.standard_normal((nq, qh, d)) * q_size, dtype), k8.bits(rng.standard_normal((nk, kvh, d)), dtype),
+            k8.bits(rng.standard_normal((nk, kvh, d)), dtype))
+
+
+def starts_of(lens):
+    return np.concatenate([[0], np.cumsum(lens)]).astype(int).tolist()
+
+
+def run(rl, q, k, v, qs, kvh, dtype, **kw):
+    n, qh, d = q.shape
+    out = k8.run_prompt(rl, q.reshape(n, -1), k.reshape(len(k), -1), v.reshape(len(v), -1), qs, qh, kvh, d, dtype, **kw)
+    return out
+
+
+@pytest.mark.parametrize("d, qh, kvh, dtype", [(128, 8, 2, "bf16"), (64, 4, 4, "fp16"), (128, 8, 1, "fp16"),
+                                               (64, 6, 2, "bf16"), (128, 2, 2, "bf16")])
+@pytest.mark.parametrize("lens", [[1], [0, 1, 2, 0], [63, 64, 65], [127, 0, 128, 129], [300, 5]])
+def test_packed(rl, gpu, d, qh, kvh, dtype, lens):
+    rng = np.random.default_rng(sum(lens) + d)
+    qs = starts_of(lens)
+    q, k, v = inputs(rng, qs[-1], qs[-1], qh, kvh, d, dtype)
+    out = run(rl, q, k, v, qs, kvh, dtype)
+    compare(out.reshape(q.shape), q, k, v, qs, qs, kvh, dtype)
+
+
+@pytest.mark.parametrize("d, qh, kvh, dtype", [(128, 16, 2, "bf16"), (64, 4, 4, "fp16")])
+def test_pieces(rl, gpu, d, qh, kvh, dtype):
+    """Queries that are the last tokens of longer sequences; a sequence with fewer keys than queries (its first queries
+    see none and yield zeros), and one without keys."""
+    rng = np.random.default_rng(7)
+    nq, nk = [1, 17, 40, 5, 3, 64], [200, 17, 333, 2, 0, 1000]
+    qs, ks = starts_of(nq), starts_of(nk)
+    q, k, v = inputs(rng, qs[-1], ks[-1], qh, kvh, d, dtype)
+    out = run(rl, q, k, v, qs, kvh, dtype, kv_starts=ks).reshape(q.shape)
+    compare(out, q, k, v, qs, ks, kvh, dtype)
+    assert not out[qs[3]:qs[3] + 3].any() and not out[qs[4]:qs[5]].any()
+
+
+@pytest.mark.parametrize("n, kvh", [(1500, 2), (2100, 1)])
+def test_long(rl, gpu, n, kvh):
+    rng = np.random.default_rng(n)
+    q, k, v = inputs(rng, n, n, 2, kvh, 128, "bf16")
+    out = run(rl, q, k, v, [0, n], kvh, "bf16").reshape(q.shape)
+    compare(out, q, k, v, [0, n], [0, n], kvh, "bf16")
+
+
+def test_few_queries_long_context(rl, gpu):
+    """One and three queries behind thousands of keys; the same bits at every replay."""
+    rng = np.random.default_rng(12)
+    nq, nk = [1, 3], [7001, 5000]
+    qs, ks = starts_of(nq), starts_of(nk)
+    q, k, v = inputs(rng, 4, ks[-1], 4, 1, 128, "bf16")
+    out = run(rl, q, k, v, qs, 1, "bf16", kv_starts=ks)
+    compare(out.reshape(q.shape), q, k, v, qs, ks, 1, "bf16")
+    assert np.array_equal(run(rl, q, k, v, qs, 1, "bf16", kv_starts=ks, graph=3), out)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_steep_scores(rl, gpu, dtype):
+    """Scores that climb along the keys (the reference maximum rises tile by tile), and large ones where a key takes all."""
+    rng = np.random.default_rng(3)
+    n, d = 400, 128
+    q, k, v = inputs(rng, n, n, 2, 1, d, dtype)
+    fk = k8.floats(k, dtype) * np.linspace(0.05, 6, n)[:, None, None]
+    fk[:, 0, 0] = np.linspace(0, 40, n)
+    fq = k8.floats(q, dtype)
+    fq[:, 0, 0] = 4.0
+    q, k = k8.bits(fq, dtype), k8.bits(fk, dtype)
+    out = run(rl, q, k, v, [0, n], 1, dtype).reshape(q.shape)
+    compare(out, q, k, v, [0, n], [0, n], 1, dtype)
+
+
+@pytest.mark.parametrize("d", [128, 64])
+def test_what_is_not_seen_has_no_part(rl, gpu, d):
+    """NaN and infinities in keys and values: rows that do not see them are as without them, rows that do are not numbers
+    where the values are not. Also in the next sequence and behind the last one."""
+    rng = np.random.default_rng(8)
+    lens, dtype = [100, 150], "bf16"
+    qs = starts_of(lens)
+    q, k, v = inputs(rng, 300, 300, 4, 2, d, dtype)
+    clean = run(rl, q, k, v, qs, 2, dtype).reshape(q.shape)
+    bad_k, bad_v = k8.floats(k, dtype), k8.floats(v, dtype)
+    bad_v[70, 0, 3] = np.nan       # sequence 0, key 70, KV head 0, dim 3
+    bad_v[90, 1, 5] = np.inf
+    bad_k[180, 1, 2] = np.nan      # sequence 1, key 80
+    bad_v[250:], bad_k[250:] = np.nan, np.inf
+    bad_k[100 + 149] = np.nan      # the last key of the last sequence
+    out = run(rl, q, k8.bits(bad_k, dtype), k8.bits(bad_v, dtype), qs, 2, dtype).reshape(q.shape)
+    f, c = k8.floats(out, dtype), k8.floats(clean, dtype)
+    tol = 3 * k8.HALF_STEP[dtype] * np.abs(c) + 2 * k8.HALF_STEP[dtype]  # (rows computed again round their weights otherwise)
+    same = np.abs(f - c) <= tol
+    assert same[:70].all() and same[100:180].all() and same[180:249, :2].all()
+    assert np.isnan(f[70:100, :2, 3]).all() and same[70:100, :2][..., np.arange(d) != 3].all()
+    assert np.isposinf(f[90:100, 2:, 5]).all() and same[90:100, 2:][..., np.arange(d) != 5].all() and same[70:90, 2:].all()
+    assert np.isnan(f[180:249, 2:]).all() and np.isnan(f[249]).all()
+
+
+def test_strides_and_bounds(rl, gpu):
+    """q, k and v as slices of one row, a wider output whose gaps stay, rows of no sequence left alone, starts past the
+    arrays cut off, a sequence longer than max_q."""
+    rng = np.random.default_rng(10)
+    d, qh, kvh, n = 64, 4, 2, 150
+    wide = (qh + 2 * kvh) * d
+    x = k8.bits(rng.standard_normal((n, wide)), "fp16")
+    q, k, v = (x[:, a * d:b * d].reshape(n, -1, d) for a, b in ((0, qh), (qh, qh + kvh), (qh + kvh, qh + 2 * kvh)))
+    qs = [10, 75, 75, 140]
+    out = k8.run_prompt(rl, x, x, x, qs, qh, kvh, d, "fp16", strides=(wide, wide, wide, qh * d + 8),
+                        offsets=(0, qh * d, (qh + kvh) * d))
+    compare(np.ascontiguousarray(out[:, :qh * d]).reshape(n, qh, d), q, k, v, qs, qs, kvh, "fp16")
+    assert (out[:, qh * d:] == 0x1234).all() and (out[:10] == 0x1234).all() and (out[140:] == 0x1234).all()
+    cut = k8.run_prompt(rl, x, x, x, [10, 75, 75, 4000], qh, kvh, d, "fp16", strides=(wide, wide, wide, qh * d + 8),
+                        offsets=(0, qh * d, (qh + kvh) * d), q_tokens=140, kv_tokens=140, max_q=65)
+    assert np.array_equal(cut, out)
+    # rows past max_q of a sequence may be left out, the others are the same
+    few = k8.run_prompt(rl, x, x, x, qs, qh, kvh, d, "fp16", strides=(wide, wide, wide, qh * d + 8),
+                        offsets=(0, qh * d, (qh + kvh) * d), max_q=33)
+    assert np.array_equal(few[10:43], out[10:43]) and np.array_equal(few[75:108], out[75:108])
+
+
+def test_nothing_to_do(rl, gpu):
+    a = rl.AttnPromptArgs(q=1 << 20, k=1 << 20, v=1 << 20, out=1 << 20, q_starts=1 << 20, seqs=1, q_tokens=0, kv_tokens=0,
+                          max_q=0, max_kv=0, q_heads=8, kv_heads=2, head_dim=64, dtype=0, workspace=1 << 20,
+                          workspace_bytes=1 << 30)
+    assert rl.lib().rl_hip_attn_prompt(C.byref(a)) == 0
+    rl.sync()
+
+
+def test_prompt_to_tokens(rl, gpu):
+    """The operators together, as a rollout uses them: the prompts' attention, their K/V into the 8-bit arena, then
+    decode steps, each attending what is cached and appending its token; every step against the model's arena."""
+    rng = np.random.default_rng(21)
+    lens, steps, qh, kvh, d, t, dtype = [37, 5, 80], 20, 8, 2, 128, 16, "bf16"
+    batch, qs = len(lens), starts_of(lens)
+    q, k, v = inputs(rng, qs[-1], qs[-1], qh, kvh, d, dtype)
+    out = run(rl, q, k, v, qs, kvh, dtype).reshape(q.shape)
+    compare(out, q, k, v, qs, qs, kvh, dtype)
+
+    need = [-(-(n + steps) // t) for n in lens]
+    stride, blocks = max(need), sum(need) * kvh
+    perm = rng.permutation(blocks).astype(np.uint32)
+    table, at = np.zeros((batch, kvh, stride), np.uint32), 0
+    for b in range(batch):
+        for g in range(kvh):
+            table[b, g, :need[b]] = perm[at:at + need[b]]
+            at += need[b]
+    model = k8.Arena8(blocks, t, d, fill=False)
+    layout, up = rl.KvLayoutDesc.paged8(t, d), rl.DeviceBuffer.from_array
+    arena = rl.Arena(blocks * layout.block_bytes, layout.block_bytes)
+    assert np.array_equal(arena.acquire_n(blocks), np.arange(blocks))
+    tb, kb, vb, sb = up(table), up(k), up(v), up(np.array(qs, np.uint32))
+    pos = up(np.zeros(batch, np.uint32))
+    fill = rl.Kv8AppendArgs(arena_base=arena.ptr, arena_bytes=arena.nbytes, layout=layout, block_table=tb.ptr,
+                            table_stride=stride, batch=batch, kv_heads=kvh, dtype=rl.DTYPE_BF16, positions=pos.ptr,
+                            starts=sb.ptr, tokens=qs[-1], max_new=max(lens), k_new=kb.ptr, v_new=vb.ptr)
+    rl.kv8_append(fill)
+    rl.sync()
+    f = [k8.floats(x, dtype) for x in (k, v)]
+    for b in range(batch):
+        for g in range(kvh):
+            s = slice(qs[b], qs[b + 1])
+            model.append(table[b, g], 0, np.stack((f[0][s, g], f[1][s, g])))
+    assert np.array_equal(arena.download(np.uint8, model.bytes.shape), model.bytes)
+
+    q1, k1, v1 = (rl.DeviceBuffer(batch * h * d * 2) for h in (qh, kvh, kvh))
+    o16, o32 = rl.DeviceBuffer(batch * qh * d * 2), rl.DeviceBuffer(batch * qh * d * 4)
+    attn = rl.attn_args(arena, layout, tb, stride, batch, qh, kvh, rl.DTYPE_BF16, pos, max(lens) + steps, q1, o16, o32)
+    ws = rl.attn_kv8_workspace(attn)
+    step_args = rl.Kv8AppendArgs(arena_base=arena.ptr, arena_bytes=arena.nbytes, layout=layout, block_table=tb.ptr,
+                                 table_stride=stride, batch=batch, kv_heads=kvh, dtype=rl.DTYPE_BF16, positions=pos.ptr,
+                                 tokens=batch, max_new=1, k_new=k1.ptr, v_new=v1.ptr)
+
+    def step():
+        rl.attn_decode_kv8(attn)
+        rl.kv8_append(step_args)
+
+    graph = rl.Graph(step)
+    for i in range(steps):
+        ctx = np.array(lens, np.uint32) + i
+        hq, hk, hv = inputs(rng, batch, batch, qh, kvh, d, dtype)
+        for dev, host in ((pos, ctx), (q1, hq), (k1, hk), (v1, hv)):
+            dev.upload(host)
+        if i % 2:
+            graph.launch()
+        else:
+            step()
+        rl.sync()
+        got = o32.download(np.float32, (batch, qh, d)).astype(float)
+        for b in range(batch):
+            for g in range(kvh):
+                kv = model.tokens(table[b, g], int(ctx[b]))
+                hs = slice(g * 4, g * 4 + 4)
+                ref, _ = k8.attend(k8.floats(hq, dtype)[b, hs], kv[0], kv[1], d ** -0.5, [int(ctx[b])] * 4)
+                assert (np.abs(got[b, hs] - ref).max(-1) <= 1e-4 * np.abs(ref).max(-1)).all(), (i, b, g)
+                model.append(table[b, g], int(ctx[b]), np.stack((k8.floats(hk, dtype)[b:b + 1, g],
+                                                                k8.floats(hv, dtype)[b:b + 1, g])))
+        assert np.array_equal(arena.download(np.uint8, model.bytes.shape), model.bytes), i
+    graph.close()
+    arena.close()
