@@ -31,6 +31,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "attn_core.h"
 #include "rl_dev_common.h"
@@ -42,6 +43,9 @@ namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int BT = 64;         // keys per tile
+constexpr int NW = 4;          // waves per workgroup, 32 rows each
+constexpr uint32_t ROWS = NW * 32;
+constexpr uint32_t kShareTiles = 8;  // tiles per workgroup, at least, where several share a row block's keys
 constexpr float kSlack = 8.f;  // log2 of what a weight may exceed its reference by
 
 struct PromptParams {
@@ -54,7 +58,11 @@ struct PromptParams {
     uint32_t pairs;   // sequences x KV heads
     uint32_t tiles;   // row blocks of the longest sequence
     uint32_t by_xcd;  // a pair's row blocks all on one XCD
+    uint32_t ranked;  // the longest sequences first
+    uint32_t seqs;
+    uint32_t split;   // workgroups per row block, at most
     float scale_log2;
+    float *part;      // [pairs x tiles][split][NW][PART] sums of split row blocks
 };
 
 template <int D>
@@ -65,6 +73,7 @@ struct PCfg {
     static constexpr int OPS = PLANE / 1024;     // 1 KiB copies per plane
     static constexpr int KS = D / 16;            // k-steps of QK
     static constexpr int DB = D / 32;            // 32-dim blocks of the output
+    static constexpr int PART = (DB * 16 + 2) * 64;  // words of a wave's sums in the workspace
     // LDS position of chunk c of row t is c ^ swizzle(t). K is read 16 rows x
     // one chunk at a time, V (transposed) four rows x four chunks.
     static __device__ __forceinline__ uint32_t kswz(uint32_t t) { return D == 128 ? t & 15u : (t >> 1) & 7u; }
@@ -113,129 +122,183 @@ __device__ __forceinline__ float half_sum(float x)
     return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
 
-template <int D, int DT, int NW>
+// The place in the batch of the sequence with the rank-th most keys (ties in
+// batch order), found by every wave for itself: p.seqs <= 64.
+__device__ __forceinline__ uint32_t seq_of_rank(const PromptParams &p, uint32_t rank, int lane)
+{
+    uint32_t n = 0;
+    if ((uint32_t)lane < p.seqs) {
+        const uint32_t a = p.kv_starts[lane], b = min(p.kv_starts[lane + 1], p.kv_tokens);
+        n = b > a ? b - a : 0u;
+    }
+    uint32_t before = 0;
+    for (uint32_t i = 0; i < p.seqs; i++) {
+        const uint32_t x = rl_readlane(n, (int)i);
+        before += x > n || (x == n && i < (uint32_t)lane) ? 1u : 0u;
+    }
+    return (uint32_t)__builtin_ctzll(__builtin_amdgcn_ballot_w64((uint32_t)lane < p.seqs && before == rank));
+}
+
+// The workgroups that share the keys of a row block of nt tiles.
+__device__ __forceinline__ uint32_t shares_of(const PromptParams &p, uint32_t nt)
+{
+    return max(1u, min(p.split, nt / kShareTiles));
+}
+
+// Which row block (of 128 rows) of which sequence and KV head workgroup `at` of
+// the grid has: the last ones, which see the most, first, the longest
+// sequences first, and all of a pair's on one XCD (workgroup b runs on XCD b %
+// 8), behind whose L2 they share K and V.
+__device__ __forceinline__ void block_of(const PromptParams &p, uint32_t at, int lane, uint32_t &seq, uint32_t &g,
+                                         uint32_t &tile)
+{
+    uint32_t pair;
+    if (p.by_xcd) {
+        const uint32_t local = at / 8;
+        pair = at % 8 + 8 * (local / p.tiles);
+        tile = p.tiles - 1 - local % p.tiles;
+    } else {
+        pair = at % p.pairs;
+        tile = p.tiles - 1 - at / p.pairs;
+    }
+    seq = pair / p.kv_heads;
+    g = pair % p.kv_heads;
+    if (p.ranked)
+        seq = seq_of_rank(p, seq, lane);
+}
+
+// One row block; SPLIT: or a share of its keys, its sums to the workspace.
+template <int D, int DT, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
 {
     using C = PCfg<D>;
     constexpr int WOPS = C::OPS / NW;  // copies of a plane per wave
     static_assert(WOPS * NW == C::OPS, "whole copies per wave");
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[2][2 * C::PLANE];
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * C::PLANE];
     const int lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t hf = (uint32_t)lane >> 5;
-
-    // heavy row blocks (the last ones) first
-    uint32_t pair, tile;
-    if (p.by_xcd) {  // workgroup b runs on XCD b % 8
-        const uint32_t local = blockIdx.x / 8;
-        pair = blockIdx.x % 8 + 8 * (local / p.tiles);
-        tile = p.tiles - 1 - local % p.tiles;
-    } else {
-        pair = blockIdx.x % p.pairs;
-        tile = p.tiles - 1 - blockIdx.x / p.pairs;
-    }
-    const uint32_t seq = pair / p.kv_heads, g = pair % p.kv_heads;
+    const uint32_t blocks = p.pairs * p.tiles, at = SPLIT ? blockIdx.x % blocks : blockIdx.x;
+    uint32_t seq, g, tile;
+    block_of(p, at, lane, seq, g, tile);
     const uint32_t qs = rl_sload(p.q_starts + seq), qe = min(rl_sload(p.q_starts + seq + 1), p.q_tokens);
     const uint32_t ks = rl_sload(p.kv_starts + seq), ke = min(rl_sload(p.kv_starts + seq + 1), p.kv_tokens);
     const uint32_t lq = qe > qs ? qe - qs : 0u, lk = ke > ks ? ke - ks : 0u;
     const uint64_t rows = (uint64_t)lq * p.group;
-    const uint64_t wg_row = (uint64_t)tile * (NW * 32);
+    const uint64_t wg_row = (uint64_t)tile * ROWS;
     if (wg_row >= rows)
         return;
     // keys that query token t sees: t + lk - lq + 1, not below 0
     auto seen = [&](uint32_t t) { return (uint32_t)max<int64_t>((int64_t)t + lk - lq + 1, 0); };
-    const uint32_t wg_seen = seen((uint32_t)(min<uint64_t>(wg_row + NW * 32, rows) - 1) / p.group);
+    const uint32_t wg_seen = seen((uint32_t)(min<uint64_t>(wg_row + ROWS, rows) - 1) / p.group);
     const uint64_t w_row = wg_row + wave * 32;
+    // this workgroup's tiles of the keys: first .. first + steps - 1
+    const uint32_t nt = (wg_seen + BT - 1) / BT;
+    uint32_t first = 0, last = nt;
+    if constexpr (SPLIT) {
+        const uint32_t n = shares_of(p, nt), share = blockIdx.x / blocks;
+        if (share >= n)
+            return;
+        first = (uint32_t)((uint64_t)share * nt / n);
+        last = (uint32_t)((uint64_t)(share + 1) * nt / n);
+    }
+    const uint32_t steps = last - first, most = (uint32_t)min<uint64_t>((uint64_t)last * BT, lk);
     const bool w_has = w_row < rows;
-    const uint32_t w_least = w_has ? seen((uint32_t)(w_row / p.group)) : 0u;
-    const uint32_t w_most = w_has ? seen((uint32_t)((min<uint64_t>(w_row + 32, rows) - 1) / p.group)) : 0u;
+    const uint32_t w_least = w_has ? min(most, seen((uint32_t)(w_row / p.group))) : 0u;
+    const uint32_t w_most = w_has ? min(most, seen((uint32_t)((min<uint64_t>(w_row + 32, rows) - 1) / p.group))) : 0u;
     const uint64_t my_row = w_row + (lane & 31);
-    const uint32_t my = (uint32_t)min<uint64_t>(my_row, rows - 1);
-    const uint32_t my_tok = my / p.group, my_head = g * p.group + my % p.group;
-    const uint32_t my_seen = seen(my_tok);
+    const uint32_t my_seen = min(most, seen((uint32_t)min<uint64_t>(my_row, rows - 1) / p.group));
+
+    // ---- the copies --------------------------------------------------------------
+    const uint16_t *kbase = p.k + (uint64_t)ks * p.k_stride + (uint64_t)g * D;
+    const uint16_t *vbase = p.v + (uint64_t)ks * p.v_stride + (uint64_t)g * D;
+    auto kbuf = [&](uint32_t s) { return (RL_LDS uint8_t *)smem + s % 2 * C::PLANE; };
+    auto vbuf = [&](uint32_t s) { return (RL_LDS uint8_t *)smem + (2 + s % 2) * C::PLANE; };
+    // row and source chunk of this lane in copy i of a plane
+    const uint32_t r0 = wave * WOPS * (64 / C::NC) + (uint32_t)lane / C::NC, pos = (uint32_t)lane % C::NC;
+    uint32_t koff[WOPS], voff[WOPS];
+#pragma unroll
+    for (int i = 0; i < WOPS; i++) {
+        const uint32_t r = r0 + i * (64 / C::NC);
+        koff[i] = r * (uint32_t)p.k_stride * 2u + ((pos ^ C::kswz(r)) << 4);
+        voff[i] = r * (uint32_t)p.v_stride * 2u + ((pos ^ C::vswz(r)) << 4);
+    }
+    // One of the wave's copies of tile t of a plane; rows past the last key
+    // repeat it (a tile that is whole needs no such look).
+    auto copy1 = [&](auto whole, const uint16_t *base, uint64_t stride, const uint32_t (&off)[WOPS], RL_LDS uint8_t *dst,
+                     uint32_t t, int i) {
+        uint32_t o = off[i];
+        if constexpr (!decltype(whole)::value) {
+            const uint32_t r = r0 + i * (64 / C::NC);
+            o -= (r - min(r, lk - t * BT - 1)) * (uint32_t)stride * 2u;
+        }
+        rl_g2lds_16_off(base + (uint64_t)t * BT * stride, o, dst + (wave * WOPS + i) * 1024);
+    };
+    // (past the last tile the copies repeat it)
+    auto copy_k = [&](auto whole, uint32_t s, int i) {
+        copy1(whole, kbase, p.k_stride, koff, kbuf(s), min(first + s, last - 1), i);
+    };
+    auto copy_v = [&](auto whole, uint32_t s, int i) {
+        copy1(whole, vbase, p.v_stride, voff, vbuf(s), min(first + s, last - 1), i);
+    };
+    constexpr std::false_type maybe{};
+    if (steps > 0)
+#pragma unroll
+        for (int i = 0; i < WOPS; i++)
+            copy_k(maybe, 0, i);
 
     s16x8 qf[C::KS];
     {
-        const uint16_t *q = p.q + (uint64_t)(qs + my_tok) * p.q_stride + (uint64_t)my_head * D + 8 * hf;
+        const uint32_t r = (uint32_t)min<uint64_t>(my_row, rows - 1);
+        const uint16_t *q = p.q + (uint64_t)(qs + r / p.group) * p.q_stride + (uint64_t)(g * p.group + r % p.group) * D + 8 * hf;
 #pragma unroll
         for (int s = 0; s < C::KS; s++)
             qf[s] = *(const s16x8 *)(q + 16 * s);
+        // Settled here: the compiler does not see the copies' waits, and would
+        // otherwise wait for these loads, and with them for the copies in
+        // flight, at their first use in every step.
+#pragma unroll
+        for (int s = 0; s < C::KS; s++)
+            asm volatile("" : "+v"(qf[s]));
     }
     f32x16 o[C::DB];
 #pragma unroll
     for (int d = 0; d < C::DB; d++)
         o[d] = f32x16{};
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, l2 = 0.f;  // (the sum in two halves)
 
-    // ---- the tiles -------------------------------------------------------------
-    const uint16_t *kbase = p.k + (uint64_t)ks * p.k_stride + (uint64_t)g * D;
-    const uint16_t *vbase = p.v + (uint64_t)ks * p.v_stride + (uint64_t)g * D;
-    auto stage = [&](uint32_t t) {
-        RL_LDS uint8_t *kd = (RL_LDS uint8_t *)smem[t & 1];
-        RL_LDS uint8_t *vd = kd + C::PLANE;
-        const uint32_t left = lk - t * BT;  // keys from this tile on; rows past them repeat the last
-        const uint16_t *kt = kbase + (uint64_t)t * BT * p.k_stride;
-        const uint16_t *vt = vbase + (uint64_t)t * BT * p.v_stride;
+    // ---- operands ----------------------------------------------------------------
+    // K: row 32 i + lane % 32, chunk 2 s + lane / 32. V: the tokens 32 i + 16 s + 4
+    // (lane / 32) .. + 3 and those 8 further, dims 32 d + lane % 32. The step's
+    // parity, the half and s are immediate offsets.
+    const uint32_t kr = (uint32_t)lane & 31u, vr = 4u * hf + (((uint32_t)lane & 15u) >> 2);
+    const uint32_t vc = 2u * (((uint32_t)lane >> 4) & 1u) + (((uint32_t)lane & 3u) >> 1);
+    RL_LDS const uint8_t *kat[C::KS], *vat[2][C::DB];
 #pragma unroll
-        for (int i = 0; i < WOPS; i++) {
-            const uint32_t op = wave * WOPS + i;
-            const uint32_t r = op * (64 / C::NC) + (uint32_t)lane / C::NC, pos = (uint32_t)lane % C::NC;
-            const uint32_t rc = min(r, left - 1);
-            rl_g2lds_16_off(kt, rc * (uint32_t)p.k_stride * 2u + ((pos ^ C::kswz(r)) << 4), kd + op * 1024);
-            rl_g2lds_16_off(vt, rc * (uint32_t)p.v_stride * 2u + ((pos ^ C::vswz(r)) << 4), vd + op * 1024);
-        }
+    for (int s = 0; s < C::KS; s++)
+        kat[s] = kbuf(0) + kr * C::RB + (((2u * s + hf) ^ C::kswz(kr)) << 4);
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int d = 0; d < C::DB; d++)
+            vat[e][d] = vbuf(0) + (vr + 8 * e) * C::RB + 8 * (lane & 1) + (((4u * d + vc) ^ C::vswz(vr + 8 * e)) << 4);
+    auto read_k = [&](int parity, int i, int s) {
+        return *(RL_LDS const s16x8 *)(kat[s] + parity * C::PLANE + 32 * i * C::RB);
     };
-    const uint32_t nt = (wg_seen + BT - 1) / BT;
-    if (nt > 0)
-        stage(0);
-    for (uint32_t t = 0; t < nt; t++) {
-        rl_wait_vmcnt<0>();
-        __syncthreads();  // tile t is there, and nobody reads tile t - 1 any more
-        if (t + 1 < nt)
-            stage(t + 1);
-        RL_LDS uint8_t *kt = (RL_LDS uint8_t *)smem[t & 1];
-        RL_LDS uint8_t *vt = kt + C::PLANE;
-        const uint32_t t0 = t * BT;
-        if (t0 + BT > lk) {  // rows past the last key: zero weights must meet zeros, not NaN
-            for (uint32_t i = threadIdx.x + (lk - t0) * C::NC; i < (uint32_t)(BT * C::NC); i += NW * 64)
-                *(RL_LDS rl_u32x4 *)(vt + i * 16) = rl_u32x4{0, 0, 0, 0};
-            __syncthreads();
-        }
-        if (t0 >= w_most)
-            continue;
-        // ---- S^T = K q^T ---------------------------------------------------------
-        f32x16 sc[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            sc[i] = f32x16{};
-            const uint32_t r = 32u * i + (lane & 31);
-            RL_LDS const uint8_t *row = kt + r * C::RB;
-#pragma unroll
-            for (int s = 0; s < C::KS; s++) {
-                const s16x8 a = *(RL_LDS const s16x8 *)(row + (((2u * s + hf) ^ C::kswz(r)) << 4));
-                sc[i] = mfma32<DT>(a, qf[s], sc[i]);
-            }
-        }
-        if (t0 + BT > w_least) {
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int r = 0; r < 16; r++)
-                    if (t0 + 32 * i + 8 * (r / 4) + 4 * hf + r % 4 >= my_seen)
-                        sc[i][r] = -INFINITY;
-        }
-        // ---- softmax -------------------------------------------------------------
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int r = 0; r < 16; r++)
-                mx = fmaxf(mx, sc[i][r]);
-        mx = half_max(mx) * p.scale_log2;
-        if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
-            const float m_new = fmaxf(m, mx);
+    auto read_v = [&](int parity, int i, int s, int d) {
+        const int at = parity * C::PLANE + (32 * i + 16 * s) * C::RB;
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((RL_LDS s16x4 *)(vat[0][d] + at));
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((RL_LDS s16x4 *)(vat[1][d] + at));
+        return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    // the scores of the keys k0 .. k0 + 31 that the row does not see
+    auto hide = [&](float x, uint32_t k0, int r) { return k0 + 8 * (r / 4) + 4 * hf + r % 4 < my_seen ? x : -INFINITY; };
+    auto raise = [&](float top) {
+        if (__builtin_amdgcn_ballot_w64(top * p.scale_log2 > m + kSlack) != 0) {
+            const float m_new = fmaxf(m, half_max(top) * p.scale_log2);
             const float alpha = m_new == -INFINITY ? 1.f : exp2f(m - m_new);
             l *= alpha;
+            l2 *= alpha;
 #pragma unroll
             for (int d = 0; d < C::DB; d++)
 #pragma unroll
@@ -243,56 +306,174 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
                     o[d][r] *= alpha;
             m = m_new;
         }
+    };
+
+    // One step: of tile t (scores in cur) the weights and V's product, of the
+    // next one the scores and their maximum. The matrix instructions, the reads
+    // of their operands AHEAD instructions earlier and the vector work are laid
+    // out here one by one: left to itself the compiler gathers each kind, and
+    // then matrix cores and vector units take turns instead of working side by
+    // side.
+    auto step = [&](auto parity_, auto masked_, f32x16 (&cur)[2], f32x16 (&next)[2], uint32_t k_next) {
+        constexpr int parity = decltype(parity_)::value;
+        constexpr bool masked = decltype(masked_)::value;
+        constexpr int PER = C::KS + 2 * C::DB;  // matrix instructions per 32 keys
+        constexpr int AHEAD = 2;
         const float neg = m == -INFINITY ? 0.f : -m;
-        s16x8 pf[4];
+        float top = -INFINITY;
+        s16x8 ring[AHEAD + 1];
+        uint32_t w[8];
+        auto fetch = [&](int n) {
+            const int i = n / PER, j = n % PER;
+            ring[n % (AHEAD + 1)] = j < C::KS ? read_k(1 - parity, i, j)
+                                              : read_v(parity, i, (j - C::KS) / C::DB, (j - C::KS) % C::DB);
+        };
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+        for (int n = 0; n < AHEAD; n++)
+            fetch(n);
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                rl_u32x4 w;
+        for (int n = 0; n < 2 * PER; n++) {
+            const int i = n / PER, j = n % PER;
+            if (j < C::KS) {
+                next[i] = mfma32<DT>(ring[n % (AHEAD + 1)], qf[j], j == 0 ? f32x16{} : next[i]);
+            } else {
+                const int u = (j - C::KS) / C::DB, d = (j - C::KS) % C::DB;
+                const s16x8 pf = __builtin_bit_cast(s16x8, (rl_u32x4{w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]}));
+                o[d] = mfma32<DT>(ring[n % (AHEAD + 1)], pf, o[d]);
+            }
+            if (n + AHEAD < 2 * PER)
+                fetch(n + AHEAD);
+            if (j < C::KS) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float a = __builtin_amdgcn_exp2f(fmaf(sc[i][8 * u + 2 * e], p.scale_log2, neg));
-                    const float b = __builtin_amdgcn_exp2f(fmaf(sc[i][8 * u + 2 * e + 1], p.scale_log2, neg));
-                    l += a + b;
+                for (int e = 8 / C::KS * j; e < 8 / C::KS * (j + 1); e++) {
+                    const float a = __builtin_amdgcn_exp2f(fmaf(cur[i][2 * e], p.scale_log2, neg));
+                    const float b = __builtin_amdgcn_exp2f(fmaf(cur[i][2 * e + 1], p.scale_log2, neg));
+                    l += a;
+                    l2 += b;
                     w[e] = pack2<DT>(a, b);
                 }
-                pf[2 * i + u] = __builtin_bit_cast(s16x8, w);
-            }
-        // ---- O^T += V^T P^T --------------------------------------------------------
+            } else {
+                constexpr int E = 16 / (2 * C::DB);
 #pragma unroll
-        for (int s = 0; s < 4; s++) {
-            const uint32_t r = 16u * s + 4u * hf + (((uint32_t)lane & 15u) >> 2);  // and r + 8
-            RL_LDS const uint8_t *row = vt + r * C::RB + 8 * (lane & 1);
-#pragma unroll
-            for (int d = 0; d < C::DB; d++) {
-                const uint32_t c = 4u * d + 2u * (((uint32_t)lane >> 4) & 1u) + (((uint32_t)lane & 3u) >> 1);
-                const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((RL_LDS s16x4 *)(row + ((c ^ C::vswz(r)) << 4)));
-                const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (RL_LDS s16x4 *)(row + 8 * C::RB + ((c ^ C::vswz(r + 8)) << 4)));
-                o[d] = mfma32<DT>(__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7), pf[s], o[d]);
+                for (int r = E * (j - C::KS); r < E * (j - C::KS + 1); r++) {
+                    if (masked)
+                        next[i][r] = hide(next[i][r], k_next + 32 * i, r);
+                    top = fmaxf(top, next[i][r]);
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        raise(top);
+    };
+
+    // ---- the tiles -------------------------------------------------------------
+    f32x16 sa[2], sb[2];
+    if (steps > 0) {
+        rl_wait_vmcnt<0>();
+        __syncthreads();  // K of step 0
+#pragma unroll
+        for (int i = 0; i < WOPS; i++)
+            copy_v(maybe, 0, i);
+#pragma unroll
+        for (int i = 0; i < WOPS; i++)
+            copy_k(maybe, 1, i);
+        if (first * BT < w_most) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                sa[i] = f32x16{};
+#pragma unroll
+                for (int s = 0; s < C::KS; s++)
+                    sa[i] = mfma32<DT>(read_k(0, i, s), qf[s], sa[i]);
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    sa[i][r] = hide(sa[i][r], first * BT + 32 * i, r);
+                    top = fmaxf(top, sa[i][r]);
+                }
+            }
+            raise(top);
         }
     }
+    // (Past a wave's last key the "next" scores are hidden whole, whatever the
+    // buffer holds.)
+    auto turn = [&](auto parity, auto masked, uint32_t s, f32x16 (&cur)[2], f32x16 (&next)[2]) {
+        const uint32_t t0 = (first + s) * BT;
+        rl_wait_vmcnt<0>();
+        rl_wait_lgkmcnt0();
+        __builtin_amdgcn_s_barrier();  // K of step s + 1 and V of step s are there; nobody reads K of step s or V of s - 1
+        asm volatile("" ::: "memory");
+        constexpr std::bool_constant<!decltype(masked)::value> whole{};
+#pragma unroll
+        for (int i = 0; i < WOPS; i++)
+            copy_k(whole, s + 2, i);
+#pragma unroll
+        for (int i = 0; i < WOPS; i++)
+            copy_v(whole, s + 1, i);
+        if (!decltype(masked)::value || t0 < w_most)
+            step(parity, masked, cur, next, t0 + BT);
+    };
+    // the steps whose next scores every row of the wave sees whole and whose copies are of whole tiles, then the rest
+    constexpr std::integral_constant<int, 0> even{};
+    constexpr std::integral_constant<int, 1> uneven{};
+    uint32_t s = 0;
+    for (; (uint64_t)(first + s + 3) * BT <= w_least && (uint64_t)(first + s + 4) * BT <= lk; s += 2) {
+        turn(even, std::false_type{}, s, sa, sb);
+        turn(uneven, std::false_type{}, s + 1, sb, sa);
+    }
+    for (; s < steps; s += 2) {
+        turn(even, std::true_type{}, s, sa, sb);
+        if (s + 1 < steps)
+            turn(uneven, std::true_type{}, s + 1, sb, sa);
+    }
+    rl_wait_vmcnt<0>();
+    const float L = half_sum(l + l2);
     // ---- the rows' outputs -------------------------------------------------------
-    const float L = half_sum(l);
-    const float inv = my_seen == 0 ? 0.f : 1.f / L;
-    uint16_t *orow = p.out + (uint64_t)(qs + my_tok) * p.out_stride + (uint64_t)my_head * D;
+    uint32_t lane_row = (uint32_t)lane & 31u;
+    asm volatile("" : "+v"(lane_row));  // (token and head are found again here, not held through the loop)
+    const uint32_t out_row = (uint32_t)min<uint64_t>(w_row + lane_row, rows - 1);
+    const uint32_t my_tok = out_row / p.group, my_head = g * p.group + out_row % p.group;
     float odd = 0.f;
 #pragma unroll
     for (int d = 0; d < C::DB; d++)
 #pragma unroll
-        for (int a = 0; a < 4; a++) {
-            rl_u32x2 w;
+        for (int r = 0; r < 16; r++)
+            odd = fmaf(o[d][r], 0.f, odd);
+    float *part = nullptr;
+    if constexpr (SPLIT)
+        part = p.part + (((size_t)at * p.split + blockIdx.x / blocks) * NW + wave) * C::PART;
+    if (SPLIT && shares_of(p, nt) > 1) {
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const float x = o[d][4 * a + 2 * e], y = o[d][4 * a + 2 * e + 1];
-                odd = fmaf(x, 0.f, fmaf(y, 0.f, odd));
-                w[e] = pack2<DT>(x * inv, y * inv);
+        for (int d = 0; d < C::DB; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                part[(16 * d + r) * 64 + lane] = o[d][r];
+        part[C::DB * 16 * 64 + lane] = m;
+        part[(C::DB * 16 + 1) * 64 + lane] = L;
+    } else {
+        // through LDS, so that a row leaves in whole lines
+        const float inv = my_seen == 0 ? 0.f : 1.f / L;
+        __syncthreads();  // the tiles' room is free
+        RL_LDS uint8_t *rows_lds = (RL_LDS uint8_t *)smem + wave * 32 * C::RB;
+        auto out_swz = [](uint32_t r) { return r & (C::NC - 1); };
+#pragma unroll
+        for (int d = 0; d < C::DB; d++)
+#pragma unroll
+            for (int a = 0; a < 4; a++) {
+                const uint32_t r = (uint32_t)lane & 31u;
+                const rl_u32x2 w = {pack2<DT>(o[d][4 * a] * inv, o[d][4 * a + 1] * inv),
+                                    pack2<DT>(o[d][4 * a + 2] * inv, o[d][4 * a + 3] * inv)};
+                *(RL_LDS rl_u32x2 *)(rows_lds + r * C::RB + (((4u * d + a) ^ out_swz(r)) << 4) + 8 * hf) = w;
             }
-            if (my_row < rows)
-                *(rl_u32x2 *)(orow + 32 * d + 8 * a + 4 * hf) = w;
+        rl_wave_lds_fence();
+#pragma unroll
+        for (int i = 0; i < C::NC / 2; i++) {
+            const uint32_t r = i * (64 / C::NC) + (uint32_t)lane / C::NC, c = (uint32_t)lane % C::NC;
+            const uint32_t tok = (uint32_t)__shfl((int)my_tok, (int)r), head = (uint32_t)__shfl((int)my_head, (int)r);
+            const rl_u32x4 w = *(RL_LDS const rl_u32x4 *)(rows_lds + r * C::RB + ((c ^ out_swz(r)) << 4));
+            if (w_row + r < rows)
+                *(rl_u32x4 *)(p.out + (uint64_t)(qs + tok) * p.out_stride + (uint64_t)head * D + c * 8) = w;
         }
+    }
     // A value of V that is no number spoils its whole 64-key tile in the matrix
     // product, also for the rows that do not see it (0 times NaN). Rows with
     // such an output are computed again, key by key, over what they see. (A
@@ -313,7 +494,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
             qv[e] = from16<DT>(q[e]);
             acc[e] = 0.f;
         }
-        for (uint32_t j = 0; j < n; j++) {
+        for (uint32_t j = first * BT; j < n; j++) {
             const uint16_t *kr = kbase + (uint64_t)j * p.k_stride + lane * E;
             const uint16_t *vr = vbase + (uint64_t)j * p.v_stride + lane * E;
             float s = 0.f;
@@ -328,6 +509,14 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
             for (int e = 0; e < E; e++)
                 acc[e] = fmaf(w, from16<DT>(vr[e]), acc[e]);
         }
+        if (SPLIT && shares_of(p, nt) > 1) {
+#pragma unroll
+            for (int e = 0; e < E; e++) {  // dim x of row r: see the merge
+                const uint32_t x = lane * E + e;
+                part[(16 * (x / 32) + 4 * (x / 8 % 4) + x % 4) * 64 + 32 * (x / 4 % 2) + r] = acc[e];
+            }
+            continue;
+        }
         uint16_t *dst = p.out + (uint64_t)(qs + tok) * p.out_stride + (uint64_t)head * D + lane * E;
 #pragma unroll
         for (int e = 0; e < E; e++)
@@ -335,25 +524,94 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     }
 }
 
-template <int D, int DT, int NW>
-int launch(PromptParams p, uint32_t seqs, uint32_t max_q)
+// Joins the shares of the row blocks that have several: wave `wave` of
+// workgroup `at` the 32 rows that wave `wave` of their workgroups had. Lane l
+// holds, of row l % 32, dim 32 d + 8 (r / 4) + 4 (l / 32) + r % 4 in word 16 d + r.
+template <int D, int DT>
+__global__ __launch_bounds__(NW * 64) void attn_prompt_merge_kernel(PromptParams p)
 {
-    p.tiles = (uint32_t)(((uint64_t)max_q * p.group + NW * 32 - 1) / (NW * 32));
-    p.pairs = seqs * p.kv_heads;
-    p.by_xcd = p.pairs % 8 == 0;
-    const uint64_t grid = (uint64_t)p.pairs * p.tiles;
-    if (grid > 0x7FFFFFFFull) {
-        rl_set_error("rl_hip_attn_prompt: %llu workgroups", (unsigned long long)grid);
-        return -1;
+    using C = PCfg<D>;
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t at = blockIdx.x / C::DB, d = blockIdx.x % C::DB;
+    uint32_t seq, g, tile;
+    block_of(p, at, lane, seq, g, tile);
+    const uint32_t qs = rl_sload(p.q_starts + seq), qe = min(rl_sload(p.q_starts + seq + 1), p.q_tokens);
+    const uint32_t ks = rl_sload(p.kv_starts + seq), ke = min(rl_sload(p.kv_starts + seq + 1), p.kv_tokens);
+    const uint32_t lq = qe > qs ? qe - qs : 0u, lk = ke > ks ? ke - ks : 0u;
+    const uint64_t rows = (uint64_t)lq * p.group;
+    const uint64_t wg_row = (uint64_t)tile * ROWS, row = wg_row + wave * 32 + (lane & 31);
+    if (wg_row >= rows)
+        return;
+    const uint32_t last_tok = (uint32_t)(min<uint64_t>(wg_row + ROWS, rows) - 1) / p.group;
+    const uint32_t wg_seen = (uint32_t)max<int64_t>((int64_t)last_tok + lk - lq + 1, 0);
+    const uint32_t n = shares_of(p, (wg_seen + BT - 1) / BT);
+    if (n < 2 || row >= rows)
+        return;
+    const float *part = p.part + ((size_t)at * p.split * NW + wave) * C::PART + lane;
+    float M = -INFINITY;
+    for (uint32_t i = 0; i < n; i++)
+        M = fmaxf(M, part[(size_t)i * NW * C::PART + C::DB * 16 * 64]);
+    float L = 0.f, o[16];
+#pragma unroll
+    for (int r = 0; r < 16; r++)
+        o[r] = 0.f;
+    for (uint32_t i = 0; i < n; i++) {
+        const float *x = part + (size_t)i * NW * C::PART;
+        const float m = x[C::DB * 16 * 64];
+        const float f = m == -INFINITY ? 0.f : exp2f(m - M);
+        L = fmaf(x[(C::DB * 16 + 1) * 64], f, L);
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+            o[r] = fmaf(x[(16 * d + r) * 64], f, o[r]);
     }
-    hipLaunchKernelGGL((attn_prompt_kernel<D, DT, NW>), dim3((uint32_t)grid), dim3(NW * 64), 0, rl_stream(), p);
-    return rl_check_launch("attn_prompt_kernel launch");
+    const uint32_t tok = (uint32_t)row / p.group, head = g * p.group + (uint32_t)row % p.group;
+    const bool none = (int64_t)tok + lk - lq + 1 <= 0;
+    const float inv = none ? 0.f : 1.f / L;
+    uint16_t *dst = p.out + (uint64_t)(qs + tok) * p.out_stride + (uint64_t)head * D + 32 * d + 4 * (lane >> 5);
+#pragma unroll
+    for (int a = 0; a < 4; a++)
+        *(rl_u32x2 *)(dst + 8 * a) = rl_u32x2{pack2<DT>(o[4 * a] * inv, o[4 * a + 1] * inv),
+                                             pack2<DT>(o[4 * a + 2] * inv, o[4 * a + 3] * inv)};
+}
+
+struct PromptPlan {
+    uint32_t tiles, pairs, split;
+    size_t workspace;
+};
+
+PromptPlan plan_of(const rl_attn_prompt_args_t *a)
+{
+    PromptPlan pl;
+    const uint32_t group = a->q_heads / a->kv_heads;
+    pl.tiles = (uint32_t)(((uint64_t)a->max_q * group + ROWS - 1) / ROWS);
+    pl.pairs = a->seqs * a->kv_heads;
+    const uint64_t blocks = (uint64_t)pl.tiles * pl.pairs;
+    const uint64_t most = std::max<uint64_t>(1, ((uint64_t)a->max_kv + BT - 1) / BT / kShareTiles);
+    pl.split = blocks == 0 ? 1 : (uint32_t)std::min<uint64_t>(most, std::max<uint64_t>(1, rl_cu_count() / blocks));
+    const size_t part = (size_t)(a->head_dim / 32 * 16 + 2) * 64 * sizeof(float);
+    pl.workspace = 256 + (pl.split > 1 ? (size_t)blocks * pl.split * NW * part : 0);
+    return pl;
 }
 
 template <int D, int DT>
-int dispatch(const PromptParams &p, uint32_t seqs, uint32_t max_q)
+int launch(const PromptParams &p)
 {
-    return launch<D, DT, 4>(p, seqs, max_q);
+    const uint64_t grid = (uint64_t)p.pairs * p.tiles * p.split;
+    if (grid > 0x7FFFFFFFull / 4) {
+        rl_set_error("rl_hip_attn_prompt: %llu workgroups", (unsigned long long)grid);
+        return -1;
+    }
+    if (p.split == 1) {
+        hipLaunchKernelGGL((attn_prompt_kernel<D, DT, false>), dim3((uint32_t)grid), dim3(NW * 64), 0, rl_stream(), p);
+        return rl_check_launch("attn_prompt_kernel launch");
+    }
+    hipLaunchKernelGGL((attn_prompt_kernel<D, DT, true>), dim3((uint32_t)grid), dim3(NW * 64), 0, rl_stream(), p);
+    if (rl_check_launch("attn_prompt_kernel launch"))
+        return -1;
+    hipLaunchKernelGGL((attn_prompt_merge_kernel<D, DT>), dim3(p.pairs * p.tiles * PCfg<D>::DB), dim3(NW * 64), 0,
+                       rl_stream(), p);
+    return rl_check_launch("attn_prompt_merge_kernel launch");
 }
 
 int validate(const rl_attn_prompt_args_t *a, const char *who)
@@ -415,7 +673,7 @@ extern "C" size_t rl_hip_attn_prompt_workspace(const rl_attn_prompt_args_t *a)
 {
     if (validate(a, "rl_hip_attn_prompt_workspace") || rl_require_open("rl_hip_attn_prompt_workspace"))
         return 0;
-    return 256;
+    return plan_of(a).workspace;
 }
 
 extern "C" int rl_hip_attn_prompt(const rl_attn_prompt_args_t *a)
@@ -425,6 +683,11 @@ extern "C" int rl_hip_attn_prompt(const rl_attn_prompt_args_t *a)
         return -1;
     if (a->max_q == 0 || a->q_tokens == 0)
         return 0;  // no query
+    const PromptPlan pl = plan_of(a);
+    if (!a->workspace || a->workspace_bytes < pl.workspace) {
+        rl_set_error("%s: workspace %zu bytes < %zu required", who, a->workspace_bytes, pl.workspace);
+        return -1;
+    }
     PromptParams p;
     p.q = (const uint16_t *)a->q;
     p.k = (const uint16_t *)a->k;
@@ -442,7 +705,14 @@ extern "C" int rl_hip_attn_prompt(const rl_attn_prompt_args_t *a)
     p.group = a->q_heads / a->kv_heads;
     const float scale = a->scale != 0.f ? a->scale : 1.0f / sqrtf((float)a->head_dim);
     p.scale_log2 = scale * 1.4426950408889634f;
+    p.seqs = a->seqs;
+    p.tiles = pl.tiles;
+    p.pairs = pl.pairs;
+    p.split = pl.split;
+    p.part = (float *)a->workspace;
+    p.by_xcd = p.pairs % 8 == 0;
+    p.ranked = p.seqs > 1 && p.seqs <= 64 && (uint64_t)p.pairs * p.tiles <= 4096;
     if (a->head_dim == 128)
-        return a->dtype == RL_DTYPE_BF16 ? dispatch<128, 0>(p, a->seqs, a->max_q) : dispatch<128, 1>(p, a->seqs, a->max_q);
-    return a->dtype == RL_DTYPE_BF16 ? dispatch<64, 0>(p, a->seqs, a->max_q) : dispatch<64, 1>(p, a->seqs, a->max_q);
+        return a->dtype == RL_DTYPE_BF16 ? launch<128, 0>(p) : launch<128, 1>(p);
+    return a->dtype == RL_DTYPE_BF16 ? launch<64, 0>(p) : launch<64, 1>(p);
 }
