@@ -7,12 +7,15 @@
 // cache, 2 head_dim per token and KV head; for few rows the chain context,
 // table, block, MFMA, merge.
 //
-//  work   a row (rollout, KV head) is ceil(ctx / 32) units of 32 tokens. A row
-//         has up to `split` workgroups that take equal shares of its units;
-//         the workgroup's waves take its units in turn.
+//  work   a row (rollout, KV head) is ceil(ctx / 32) units of 32 tokens. Few
+//         rows have workgroups of their own, many rows are cut in even shares
+//         (the two kernels below); a workgroup's waves take its units in turn.
 //  loads  straight to registers, one unit ahead of the one that is consumed:
 //         no LDS, no barriers in the loop. A lane's K bytes are one token's,
-//         its V bytes eight tokens'.
+//         its V bytes eight tokens'. Every load of the loop is a vector load,
+//         counted in order: scalar loads of the scales, which return in any
+//         order, cost the whole latency per unit (124 us against 102 at 8 x
+//         32,768 tokens).
 //  QK     v_mfma_f32_16x16x32: A = 16 tokens' K, B = q^T with the heads of the
 //         group as columns (up to 16). A lane's 16 consecutive K bytes are two
 //         k-steps of the product; q's dims are permuted the same way. The
@@ -39,8 +42,8 @@
 namespace {
 
 constexpr int kUnit = 32;           // tokens per unit
-constexpr uint32_t kMaxSplit = 64;  // workgroups per row at most
-constexpr int kWavesPerWg = 4;
+constexpr uint32_t kRowCost = 8;    // units that turning to a row is worth
+
 
 struct Kv8Params {
     const uint8_t *arena;
@@ -50,20 +53,31 @@ struct Kv8Params {
     uint32_t table_stride;
     const uint32_t *ctx;
     uint32_t max_ctx;
+    uint32_t batch;
     uint32_t q_heads, kv_heads, group;
     const uint16_t *q;
     uint16_t *out;
     float *out_f32;
     float scale_log2;
-    uint32_t split;      // workgroups per row
-    uint32_t min_units;  // units per workgroup, at least, where a row has several
-    float *part;         // [rows][split][group * D + 2 * group]
+    uint32_t split;      // rows kernel: workgroups per row; even kernel: workgroups
+    uint32_t min_units;  // units per workgroup, at least, where there are several
+    float *part;         // partials, [group * D + 2 * group] each
+    uint32_t *cum;       // even kernel: [batch + 1] units of all rows before rollout b
 };
 
-// The workgroups that share a row of nu units.
-__device__ __forceinline__ uint32_t row_wgs(const Kv8Params &p, uint32_t nu)
+__device__ __forceinline__ uint32_t units_of(const Kv8Params &p, uint32_t ctx)
 {
-    return max(1u, min(p.split, nu / p.min_units));
+    return (uint32_t)(((uint64_t)min(ctx, p.max_ctx) + kUnit - 1) / kUnit);
+}
+
+// What a row costs a workgroup, in units: its units, and the latencies of
+// turning to it.
+__device__ __forceinline__ uint32_t cost_of(uint32_t units) { return units ? units + kRowCost : 0u; }
+
+// Of the workgroups there are, those that share n units.
+__device__ __forceinline__ uint32_t sharing(const Kv8Params &p, uint32_t n)
+{
+    return max(1u, min(p.split, n / p.min_units));
 }
 
 // One unit as it was loaded: K of two 16-token tiles, V of eight tokens per
@@ -178,37 +192,46 @@ __device__ __forceinline__ uint32_t xcd_contiguous(uint32_t n)
     return n % 8 != 0 ? blockIdx.x : (blockIdx.x % 8) * (n / 8) + blockIdx.x / 8;
 }
 
+// The table entries of 64 of a wave's units (one per lane), from its first-th on:
+// units u0 + wave, u0 + wave + W, ... of a row. They are asked for without a look
+// at the context; what lies past it is never used.
+template <int TPB>
+struct Window8 {
+    uint32_t e[kUnit / TPB];
+};
+
+template <int TPB, int W>
+__device__ __forceinline__ Window8<TPB> window8(const Kv8Params &p, uint32_t row, uint32_t u0, uint32_t first)
+{
+    constexpr int BPU = kUnit / TPB;  // blocks per unit
+    const uint32_t *trow = p.table + (size_t)row * p.table_stride;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Window8<TPB> win;
+#pragma unroll
+    for (int i = 0; i < BPU; i++) {
+        const uint64_t at = ((uint64_t)u0 + wave + (uint64_t)(first + (threadIdx.x & 63)) * W) * BPU + i;
+        win.e[i] = at < p.table_stride ? trow[at] : 0u;
+    }
+    return win;
+}
+
+// Units u0 .. u1 - 1 of row (rollout b, KV head g) by the W waves of a
+// workgroup: the row's output when part is NULL, else a partial. lds: [W][G * D
+// + 2 G] floats, free again when the last wave returns from a later barrier.
+// win: the wave's first table entries (window8), loaded by the caller as early
+// as it can.
 template <int D, int DT, int TPB, int W>
-__global__ __launch_bounds__(W * 64) void attn_kv8_kernel(Kv8Params p)
+__device__ __forceinline__ void attend8(const Kv8Params &p, uint32_t b, uint32_t g, uint32_t cin, uint32_t u0,
+                                        uint32_t u1, Window8<TPB> win, float *part, float *lds)
 {
     constexpr int BPU = kUnit / TPB;  // blocks per unit
     constexpr int NJ = D / 16;
-    extern __shared__ float lds[];    // [W][G * D + 2 G]
     const int lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t wg = xcd_contiguous(gridDim.x);
-    const uint32_t row = wg / p.split, s = wg % p.split;
-    const uint32_t b = row / p.kv_heads, g = row % p.kv_heads, G = p.group;
     const int h = lane & 15, c = lane >> 4;
-    const uint32_t PART = G * D + 2 * G;
-
-    const uint32_t cin = rl_sload(p.ctx + b);
+    const uint32_t G = p.group, PART = G * D + 2 * G, row = b * p.kv_heads + g;
     const uint32_t ctx = min(cin, p.max_ctx);
-    const uint32_t nu = (uint32_t)(((uint64_t)ctx + kUnit - 1) / kUnit);
-    const uint32_t nwg = row_wgs(p, nu);
-    if (s >= nwg)
-        return;
     const size_t obase = ((size_t)b * p.q_heads + (size_t)g * G) * D;
-    if (nu == 0) {  // no token: zeros (NaN where max_ctx is 0 and the context is not)
-        for (uint32_t e = threadIdx.x; e < G * D; e += W * 64) {
-            const float v = cin > p.max_ctx ? __builtin_nanf("") : 0.f;
-            p.out[obase + e] = rl_from_f32<DT>(v);
-            if (p.out_f32)
-                p.out_f32[obase + e] = v;
-        }
-        return;
-    }
-    const uint32_t u0 = (uint32_t)((uint64_t)s * nu / nwg), u1 = (uint32_t)((uint64_t)(s + 1) * nu / nwg);
     const uint32_t n = u1 - u0 > wave ? (u1 - u0 - wave + W - 1) / W : 0u;  // this wave's units
     bool bad = cin > p.max_ctx;
 
@@ -220,19 +243,7 @@ __global__ __launch_bounds__(W * 64) void attn_kv8_kernel(Kv8Params p)
         rs.acc[j] = rl_f32x4{0.f, 0.f, 0.f, 0.f};
 
     if (n > 0) {
-        const uint32_t *trow = p.table + (size_t)row * p.table_stride;
         const uint32_t nblk = (uint32_t)(((uint64_t)ctx + TPB - 1) / TPB);
-        uint32_t win[BPU], wfirst = 0;
-        auto window = [&](uint32_t first) {
-            wfirst = first;
-#pragma unroll
-            for (int i = 0; i < BPU; i++) {
-                const uint64_t at = ((uint64_t)u0 + wave + (uint64_t)(first + lane) * W) * BPU + i;
-                // (the last unit's second block may not exist: its first one again, all masked)
-                win[i] = at < nblk ? trow[at] : (i > 0 && at == nblk ? trow[at - 1] : 0u);
-            }
-        };
-        window(0);
         {
             const int hq = min(h, (int)G - 1);
             const uint16_t *q = p.q + obase + (size_t)hq * D;
@@ -242,17 +253,36 @@ __global__ __launch_bounds__(W * 64) void attn_kv8_kernel(Kv8Params p)
                 rs.qf[t] = h < (int)G ? v : s16x8{0, 0, 0, 0, 0, 0, 0, 0};
             }
         }
+        uint32_t wfirst = 0;
+        // Settled once per 64 units: else every reading of an entry would wait
+        // for all loads in flight. The last unit's second block may not exist:
+        // its first one again, all masked.
+        auto settle = [&] {
+#pragma unroll
+            for (int i = 0; i < BPU; i++)
+                asm volatile("" : "+v"(win.e[i]));
+            if constexpr (BPU == 2) {
+                const uint64_t at = ((uint64_t)u0 + wave + (uint64_t)(wfirst + lane) * W) * 2 + 1;
+                win.e[BPU - 1] = at < nblk ? win.e[BPU - 1] : win.e[0];
+            }
+        };
+        settle();
         const uint32_t koff = (uint32_t)h * D + 16u * c;
+        uint32_t zero = 0;
+        asm volatile("" : "+v"(zero));
         const uint32_t voff = (uint32_t)TPB * D + 4u * c * D + (uint32_t)h * NJ;
         auto load = [&](uint32_t k, Unit<D> &u) {
             k = min(k, n - 1);
-            if (k - wfirst >= 64u)
-                window(k);
+            if (k - wfirst >= 64u) {
+                wfirst = k;
+                win = window8<TPB, W>(p, row, u0, k);
+                settle();
+            }
             u.bad = false;
             const uint8_t *base[BPU];
 #pragma unroll
             for (int i = 0; i < BPU; i++) {
-                uint32_t blk = rl_readlane(win[i], (int)(k - wfirst));
+                uint32_t blk = rl_readlane(win.e[i], (int)(k - wfirst));
                 if (blk >= p.arena_blocks) {  // never read outside the arena
                     u.bad = true;
                     blk = 0;
@@ -265,7 +295,8 @@ __global__ __launch_bounds__(W * 64) void attn_kv8_kernel(Kv8Params p)
 #pragma unroll
                 for (int q = 0; q < D / 64; q++)
                     u.k[i][q] = *(const rl_u32x4 *)(at + koff + 64 * q);
-                u.scale[i] = rl_sload((const rl_f32x2 *)(base[i % BPU] + 2 * TPB * D));
+                // (a vector load: these return in order, so the unit in flight is not waited for)
+                u.scale[i] = *(const rl_f32x2 *)(base[i % BPU] + 2 * TPB * D + zero);
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -336,8 +367,7 @@ __global__ __launch_bounds__(W * 64) void attn_kv8_kernel(Kv8Params p)
             L += lds[i * PART + G * D + 2 * hh + 1] * f;
             O += lds[i * PART + e] * f;
         }
-        if (nwg > 1) {
-            float *part = p.part + ((size_t)row * p.split + s) * PART;
+        if (part) {
             part[e] = O;
             if (e % D == 0) {
                 part[G * D + 2 * hh] = M;
@@ -352,33 +382,162 @@ __global__ __launch_bounds__(W * 64) void attn_kv8_kernel(Kv8Params p)
     }
 }
 
+// A row without tokens: zeros (NaN where max_ctx is 0 and the context is not).
+template <int D, int DT>
+__device__ __forceinline__ void empty8(const Kv8Params &p, uint32_t b, uint32_t g, uint32_t cin, uint32_t e)
+{
+    const size_t at = ((size_t)b * p.q_heads + (size_t)g * p.group) * D + e;
+    const float v = cin > p.max_ctx ? __builtin_nanf("") : 0.f;
+    p.out[at] = rl_from_f32<DT>(v);
+    if (p.out_f32)
+        p.out_f32[at] = v;
+}
+
+// ---- few rows: workgroups that own their rows ----------------------------------
+// `split` workgroups per row. Nothing but the row's own context decides its
+// work, so the chain of loads is short: context, table, units.
+template <int D, int DT, int TPB, int W>
+__global__ __launch_bounds__(W * 64) void attn_kv8_rows_kernel(Kv8Params p)
+{
+    extern __shared__ float lds[];
+    const uint32_t wg = xcd_contiguous(gridDim.x);
+    const uint32_t row = wg / p.split, s = wg % p.split;
+    const uint32_t b = row / p.kv_heads, g = row % p.kv_heads;
+    Window8<TPB> win;
+    if (p.split == 1)  // the row's first units are this workgroup's, whatever the context
+        win = window8<TPB, W>(p, row, 0, 0);
+    const uint32_t cin = rl_sload(p.ctx + b), nu = units_of(p, cin), n = sharing(p, nu);
+    if (s >= n)
+        return;
+    if (nu == 0) {
+        for (uint32_t e = threadIdx.x; e < p.group * D; e += W * 64)
+            empty8<D, DT>(p, b, g, cin, e);
+        return;
+    }
+    const uint32_t u0 = (uint32_t)((uint64_t)s * nu / n), u1 = (uint32_t)((uint64_t)(s + 1) * nu / n);
+    if (p.split > 1)
+        win = window8<TPB, W>(p, row, u0, 0);
+    attend8<D, DT, TPB, W>(p, b, g, cin, u0, u1, win,
+                           n > 1 ? p.part + (size_t)wg * (p.group * D + 2 * p.group) : nullptr, lds);
+}
+
+// ---- many rows: the units of all rows in even shares -----------------------------
+// The units of all rows, rows in (b, g) order, form one sequence; the
+// workgroups, two per compute unit, take equal runs of it, whatever the
+// contexts are. A run that covers a row writes its output; a row that several
+// share is merged from their partials. A workgroup has at most two of those, of
+// the rows its run starts and ends in: number 2 w when the row's part starts
+// the run, else 2 w + 1.
+template <int D, int DT, int TPB, int W>
+__global__ __launch_bounds__(W * 64) void attn_kv8_even_kernel(Kv8Params p)
+{
+    extern __shared__ float lds[];
+    const int lane = threadIdx.x & 63;
+    const uint32_t wg = xcd_contiguous(gridDim.x);
+    const uint32_t PART = p.group * D + 2 * p.group;
+    auto cost64 = [&](uint32_t b0) {  // of the rows of rollout b0 + lane
+        return b0 + lane < p.batch ? cost_of(units_of(p, p.ctx[b0 + lane])) * p.kv_heads : 0u;
+    };
+    const uint32_t t0 = cost64(0);
+    uint32_t total = rl_wave_sum_u32(t0);
+    for (uint32_t b0 = 64; b0 < p.batch; b0 += 64)
+        total += rl_wave_sum_u32(cost64(b0));
+    const uint32_t n = sharing(p, total);
+    const uint32_t first = (uint32_t)((uint64_t)wg * total / n), last = (uint32_t)((uint64_t)(wg + 1) * total / n);
+    // (the wave, not its threads, decides: what follows stays in scalar registers)
+    const bool writes = wg == 0 && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) == 0;
+    // the rollout that the run begins in, and the cost before it
+    uint32_t b = 0, before = 0, sum = 0;
+    bool found = false;
+    for (uint32_t b0 = 0; b0 < p.batch && (writes || !found); b0 += 64) {
+        const uint32_t t = b0 == 0 ? t0 : cost64(b0);
+        const uint32_t inc = sum + rl_wave_incl_scan_u32(t);
+        if (writes && b0 + lane < p.batch)
+            p.cum[b0 + lane] = inc - t;
+        const uint64_t in = __builtin_amdgcn_ballot_w64(inc > first);
+        if (!found && in) {
+            const int l = __builtin_ctzll(in);
+            found = true;
+            b = b0 + l;
+            before = rl_readlane(inc - t, l);
+        }
+        sum = rl_readlane(inc, 63);
+    }
+    if (writes && lane == 0)
+        p.cum[p.batch] = total;
+    if (wg >= n || total == 0)
+        return;
+    uint32_t cin = rl_sload(p.ctx + b), nu = units_of(p, cin);
+    uint32_t g = (first - before) / cost_of(nu), x = (first - before) % cost_of(nu);  // x: of this row's cost
+    uint32_t parts = 0;
+    for (uint32_t at = first; at < last;) {
+        const uint32_t m = min(cost_of(nu) - x, last - at);
+        const uint32_t u0 = max(x, kRowCost) - kRowCost, u1 = max(x + m, kRowCost) - kRowCost;
+        if (u1 > u0) {
+            attend8<D, DT, TPB, W>(p, b, g, cin, u0, u1, window8<TPB, W>(p, b * p.kv_heads + g, u0, 0),
+                                   u1 - u0 < nu ? p.part + (size_t)(2 * wg + min(parts, 1u)) * PART : nullptr, lds);
+            parts++;
+            __syncthreads();
+        }
+        at += m;
+        x = 0;
+        if (++g == p.kv_heads && at < last) {
+            g = 0;
+            do {
+                cin = rl_sload(p.ctx + ++b);
+                nu = units_of(p, cin);
+            } while (nu == 0);  // (cost remains, so a later rollout has some)
+        }
+    }
+}
+
 // Merges the partials of the rows that several workgroups shared: thread e of
 // workgroup (x, row) output element 256 x + e of the row.
-template <int DT, int D>
+template <int D, int DT, bool EVEN>
 __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8Params p)
 {
     const uint32_t G = p.group, PART = G * D + 2 * G, NE = G * D;
     const uint32_t blocks = (NE + 255) / 256;
     const uint32_t row = blockIdx.x / blocks, e = blockIdx.x % blocks * 256 + threadIdx.x;
     const uint32_t b = row / p.kv_heads, g = row % p.kv_heads;
-    const uint32_t cin = rl_sload(p.ctx + b);
-    const uint32_t nwg = row_wgs(p, (uint32_t)(((uint64_t)min(cin, p.max_ctx) + kUnit - 1) / kUnit));
-    if (nwg < 2 || e >= NE)
+    const uint32_t cin = rl_sload(p.ctx + b), nu = units_of(p, cin);
+    if (e >= NE)
         return;
-    const float *part = p.part + (size_t)row * p.split * PART;
+    const float *part, *start;  // the later ones follow each other, the first may lie elsewhere
+    uint32_t n, step;
+    if constexpr (EVEN) {
+        if (nu == 0) {
+            empty8<D, DT>(p, b, g, cin, e);
+            return;
+        }
+        // the places of the row's units in the sequence, and of the runs that hold the first and the last
+        const uint32_t total = rl_sload(p.cum + p.batch), row0 = rl_sload(p.cum + b) + g * cost_of(nu);
+        const uint64_t wgs = sharing(p, total), r0 = (uint64_t)row0 + kRowCost;
+        const uint32_t w0 = (uint32_t)(((r0 + 1) * wgs - 1) / total), w1 = (uint32_t)(((r0 + nu) * wgs - 1) / total);
+        n = w1 - w0 + 1;
+        step = 2 * PART;
+        part = p.part + (size_t)w0 * step;
+        start = part + ((uint64_t)w0 * total / wgs < row0 ? PART : 0u);
+    } else {
+        n = sharing(p, nu);
+        step = PART;
+        start = part = p.part + (size_t)row * p.split * PART;
+    }
+    if (n < 2)
+        return;
     float M = -INFINITY, L = 0.f, O = 0.f;
-    for (uint32_t i0 = 0; i0 < nwg; i0 += 8) {
+    for (uint32_t i0 = 0; i0 < n; i0 += 8) {
         float o[8], mm[8], ll[8], mx = M;
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {
-            const float *pp = part + (size_t)min(i0 + i, nwg - 1) * PART;
+            const float *pp = i0 + i == 0 ? start : part + (size_t)min(i0 + i, n - 1) * step;
             o[i] = pp[e];
             mm[i] = pp[NE + 2 * (e / D)];
             ll[i] = pp[NE + 2 * (e / D) + 1];
         }
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {
-            mm[i] = i0 + i < nwg ? mm[i] : -INFINITY;
+            mm[i] = i0 + i < n ? mm[i] : -INFINITY;
             mx = fmaxf(mx, mm[i]);
         }
         const float keep = M == -INFINITY ? 0.f : exp2f(M - mx);
@@ -388,8 +547,8 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8Params p)
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {
             const float f = mm[i] == -INFINITY ? 0.f : exp2f(mm[i] - M);
-            L = i0 + i < nwg ? L + ll[i] * f : L;
-            O = i0 + i < nwg ? O + o[i] * f : O;
+            L = i0 + i < n ? L + ll[i] * f : L;
+            O = i0 + i < n ? O + o[i] * f : O;
         }
     }
     const float v = O / L;
@@ -401,48 +560,82 @@ __global__ __launch_bounds__(256) void attn_kv8_merge_kernel(Kv8Params p)
 
 // ---- launcher ------------------------------------------------------------------
 
+// Which kernel and how many workgroups, by sizes alone (times in us, GQA 4,
+// 8 KV heads, d128 unless said):
+//  - the even shares from 100 units of the longest context and 16,384 units in
+//    all on: 16 x 4,000-16,000 tokens 68.2 against 73.4 of the rows kernel, 64 x
+//    1-4,000 59.7 against 64.7, 128 x 512-4,096 122 against 127; below, turning to
+//    the next row costs more than uneven rows do: 64 x 512-2,048 43.4 against
+//    39.8, 128 x 64-1,024 43.2 against 37.4, 256 x 100-200 39.0 against 27.3.
+//  - rows of few units whole, in one launch: 1 x 517 tokens (17 units) 8.1
+//    against 9.2 with the row in two.
+//  - one row per compute unit, with eight waves: 24 x 64-2,048 tokens of d64,
+//    192 rows, 11.4 against 12.6 with four waves and rows in two.
+//  - else as many workgroups per row as two per compute unit allow, of 8 units
+//    and more: 1 x 1,024 9.4 against 10.6 with 16 and more, 4 x 100-1,024 10.4
+//    against 11.7.
+constexpr uint64_t kEvenContext = 100, kEvenUnits = 16384, kWholeUnits = 24, kShareUnits = 8;
+
 struct Plan8 {
-    uint32_t split, min_units;
+    bool even;
+    uint32_t split, min_units, waves;
+    size_t part_off, total;  // of the workspace
 };
 
 Plan8 plan_of(const rl_attn_decode_args_t *a)
 {
     Plan8 pl;
-    pl.min_units = 2 * kWavesPerWg;
     const uint64_t rows = (uint64_t)a->batch * a->kv_heads;
-    const uint64_t most = std::max<uint64_t>(1, ((uint64_t)a->max_ctx + kUnit - 1) / kUnit / pl.min_units);
-    const uint64_t want = std::max<uint64_t>(1, 4096 / rows);
-    pl.split = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(most, want), kMaxSplit);
+    const uint64_t units = std::max<uint64_t>(1, ((uint64_t)a->max_ctx + kUnit - 1) / kUnit);
+    const uint32_t cus = rl_cu_count();
+    pl.waves = 4;
+    pl.even = units >= kEvenContext && rows * units >= kEvenUnits;
+    pl.min_units = kShareUnits;
+    if (pl.even) {
+        pl.split = 2 * cus;
+    } else if (rows > cus / 2 && rows <= cus && units >= kWholeUnits) {
+        pl.split = 1;
+        pl.waves = 8;
+    } else {
+        const uint64_t most = units < kWholeUnits ? 1 : units / pl.min_units;
+        pl.split = (uint32_t)std::min<uint64_t>(most, std::max<uint64_t>(1, 2 * cus / rows));
+    }
+    const uint32_t G = a->q_heads / a->kv_heads;
+    const size_t part = (size_t)(G * a->layout.head_dim + 2 * G) * sizeof(float);
+    pl.part_off = pl.even ? (((size_t)a->batch + 1) * 4 + 255) / 256 * 256 : 0;
+    pl.total = 256 + pl.part_off + (pl.even ? 2 * (size_t)pl.split * part : pl.split > 1 ? rows * pl.split * part : 0);
     return pl;
 }
 
-size_t workspace_of(const rl_attn_decode_args_t *a)
-{
-    const uint32_t G = a->q_heads / a->kv_heads;
-    const Plan8 pl = plan_of(a);
-    const size_t rows = (size_t)a->batch * a->kv_heads;
-    return 256 + (pl.split > 1 ? rows * pl.split * (G * a->layout.head_dim + 2 * G) * sizeof(float) : 0);
-}
-
 template <int D, int DT, int TPB>
-int launch(const Kv8Params &p, uint64_t rows)
+int launch(const Kv8Params &p, uint64_t rows, const Plan8 &pl)
 {
-    const size_t lds = (size_t)kWavesPerWg * (p.group * D + 2 * p.group) * sizeof(float);
-    hipLaunchKernelGGL((attn_kv8_kernel<D, DT, TPB, kWavesPerWg>), dim3((uint32_t)(rows * p.split)),
-                       dim3(kWavesPerWg * 64), lds, rl_stream(), p);
-    if (rl_check_launch("attn_kv8_kernel launch"))
+    const size_t lds = (size_t)pl.waves * (p.group * D + 2 * p.group) * sizeof(float);
+    const dim3 threads(pl.waves * 64), merge((uint32_t)(rows * ((p.group * D + 255) / 256)));
+    if (pl.even) {
+        hipLaunchKernelGGL((attn_kv8_even_kernel<D, DT, TPB, 4>), dim3(p.split), threads, lds, rl_stream(), p);
+        if (rl_check_launch("attn_kv8_even_kernel launch"))
+            return -1;
+        hipLaunchKernelGGL((attn_kv8_merge_kernel<D, DT, true>), merge, dim3(256), 0, rl_stream(), p);
+        return rl_check_launch("attn_kv8_merge_kernel launch");
+    }
+    const dim3 grid((uint32_t)(rows * p.split));
+    if (pl.waves == 8)
+        hipLaunchKernelGGL((attn_kv8_rows_kernel<D, DT, TPB, 8>), grid, threads, lds, rl_stream(), p);
+    else
+        hipLaunchKernelGGL((attn_kv8_rows_kernel<D, DT, TPB, 4>), grid, threads, lds, rl_stream(), p);
+    if (rl_check_launch("attn_kv8_rows_kernel launch"))
         return -1;
     if (p.split < 2)
         return 0;
-    const uint32_t blocks = (p.group * D + 255) / 256;
-    hipLaunchKernelGGL((attn_kv8_merge_kernel<DT, D>), dim3((uint32_t)(rows * blocks)), dim3(256), 0, rl_stream(), p);
+    hipLaunchKernelGGL((attn_kv8_merge_kernel<D, DT, false>), merge, dim3(256), 0, rl_stream(), p);
     return rl_check_launch("attn_kv8_merge_kernel launch");
 }
 
 template <int D, int DT>
-int dispatch(const Kv8Params &p, uint64_t rows, uint32_t tpb)
+int dispatch(const Kv8Params &p, uint64_t rows, const Plan8 &pl, uint32_t tpb)
 {
-    return tpb == 16 ? launch<D, DT, 16>(p, rows) : launch<D, DT, 32>(p, rows);
+    return tpb == 16 ? launch<D, DT, 16>(p, rows, pl) : launch<D, DT, 32>(p, rows, pl);
 }
 
 int validate(const rl_attn_decode_args_t *a, const char *who)
@@ -484,6 +677,11 @@ int validate(const rl_attn_decode_args_t *a, const char *who)
         rl_set_error("%s: grid_waves %u (only 0, the library's own split)", who, a->grid_waves);
         return -1;
     }
+    if ((uint64_t)a->batch * a->kv_heads * (((uint64_t)a->max_ctx + kUnit - 1) / kUnit) >= (1ull << 32)) {
+        rl_set_error("%s: batch %u x kv_heads %u of max_ctx %u exceeds 2^32 units of %d tokens", who, a->batch,
+                     a->kv_heads, a->max_ctx, kUnit);
+        return -1;
+    }
     const uint64_t table_need = ((uint64_t)a->max_ctx + a->layout.token_count - 1) / a->layout.token_count;
     if (a->table_stride < table_need) {
         rl_set_error("%s: table_stride %u < %llu blocks needed for max_ctx %u", who, a->table_stride,
@@ -499,7 +697,7 @@ extern "C" size_t rl_hip_attn_decode_kv8_workspace(const rl_attn_decode_args_t *
 {
     if (validate(a, "rl_hip_attn_decode_kv8_workspace") || rl_require_open("rl_hip_attn_decode_kv8_workspace"))
         return 0;
-    return workspace_of(a);
+    return plan_of(a).total;
 }
 
 extern "C" int rl_hip_attn_decode_kv8(const rl_attn_decode_args_t *a)
@@ -507,12 +705,11 @@ extern "C" int rl_hip_attn_decode_kv8(const rl_attn_decode_args_t *a)
     const char *who = "rl_hip_attn_decode_kv8";
     if (validate(a, who) || rl_require_open(who))
         return -1;
-    const size_t need = workspace_of(a);
-    if (!a->workspace || a->workspace_bytes < need) {
-        rl_set_error("%s: workspace %zu bytes < %zu required", who, a->workspace_bytes, need);
+    const Plan8 pl = plan_of(a);
+    if (!a->workspace || a->workspace_bytes < pl.total) {
+        rl_set_error("%s: workspace %zu bytes < %zu required", who, a->workspace_bytes, pl.total);
         return -1;
     }
-    const Plan8 pl = plan_of(a);
     Kv8Params p;
     p.arena = (const uint8_t *)a->arena_base;
     p.block_bytes = a->layout.block_bytes;
@@ -521,6 +718,7 @@ extern "C" int rl_hip_attn_decode_kv8(const rl_attn_decode_args_t *a)
     p.table_stride = a->table_stride;
     p.ctx = a->ctx_lens;
     p.max_ctx = a->max_ctx;
+    p.batch = a->batch;
     p.q_heads = a->q_heads;
     p.kv_heads = a->kv_heads;
     p.group = a->q_heads / a->kv_heads;
@@ -531,10 +729,11 @@ extern "C" int rl_hip_attn_decode_kv8(const rl_attn_decode_args_t *a)
     p.scale_log2 = scale * 1.4426950408889634f;
     p.split = pl.split;
     p.min_units = pl.min_units;
-    p.part = (float *)a->workspace;
+    p.cum = (uint32_t *)a->workspace;
+    p.part = (float *)((uint8_t *)a->workspace + pl.part_off);
     const uint64_t rows = (uint64_t)a->batch * a->kv_heads;
     const uint32_t tpb = a->layout.token_count;
     if (a->layout.head_dim == 128)
-        return a->dtype == RL_DTYPE_BF16 ? dispatch<128, 0>(p, rows, tpb) : dispatch<128, 1>(p, rows, tpb);
-    return a->dtype == RL_DTYPE_BF16 ? dispatch<64, 0>(p, rows, tpb) : dispatch<64, 1>(p, rows, tpb);
+        return a->dtype == RL_DTYPE_BF16 ? dispatch<128, 0>(p, rows, pl, tpb) : dispatch<128, 1>(p, rows, pl, tpb);
+    return a->dtype == RL_DTYPE_BF16 ? dispatch<64, 0>(p, rows, pl, tpb) : dispatch<64, 1>(p, rows, pl, tpb);
 }
