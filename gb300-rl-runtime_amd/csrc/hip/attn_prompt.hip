@@ -46,6 +46,7 @@ constexpr int BT = 64;         // keys per tile
 constexpr int NW = 4;          // waves per workgroup, 32 rows each
 constexpr uint32_t ROWS = NW * 32;
 constexpr uint32_t kShareTiles = 8;  // tiles per workgroup, at least, where several share a row block's keys
+constexpr int kPlain = 0, kMasked = 1, kFinal = 2;  // what a step's next scores are: all seen, some hidden, none
 constexpr float kSlack = 8.f;  // log2 of what a weight may exceed its reference by
 
 struct PromptParams {
@@ -314,10 +315,11 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     // out here one by one: left to itself the compiler gathers each kind, and
     // then matrix cores and vector units take turns instead of working side by
     // side.
-    auto step = [&](auto parity_, auto masked_, f32x16 (&cur)[2], f32x16 (&next)[2], uint32_t k_next) {
+    auto step = [&](auto parity_, auto kind_, f32x16 (&cur)[2], f32x16 (&next)[2], uint32_t k_next) {
         constexpr int parity = decltype(parity_)::value;
-        constexpr bool masked = decltype(masked_)::value;
-        constexpr int PER = C::KS + 2 * C::DB;  // matrix instructions per 32 keys
+        constexpr int kind = decltype(kind_)::value;
+        constexpr int QK = kind == kFinal ? 0 : C::KS;  // matrix instructions per 32 keys: of the next scores, ...
+        constexpr int PER = QK + 2 * C::DB;              // ... and in all
         constexpr int AHEAD = 2;
         const float neg = m == -INFINITY ? 0.f : -m;
         float top = -INFINITY;
@@ -325,8 +327,18 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
         uint32_t w[8];
         auto fetch = [&](int n) {
             const int i = n / PER, j = n % PER;
-            ring[n % (AHEAD + 1)] = j < C::KS ? read_k(1 - parity, i, j)
-                                              : read_v(parity, i, (j - C::KS) / C::DB, (j - C::KS) % C::DB);
+            ring[n % (AHEAD + 1)] = j < QK ? read_k(1 - parity, i, j) : read_v(parity, i, (j - QK) / C::DB, (j - QK) % C::DB);
+        };
+        // the pairs e0 .. e1 - 1 of the weights of half i
+        auto weights = [&](int i, int e0, int e1) {
+#pragma unroll
+            for (int e = e0; e < e1; e++) {
+                const float a = __builtin_amdgcn_exp2f(fmaf(cur[i][2 * e], p.scale_log2, neg));
+                const float b = __builtin_amdgcn_exp2f(fmaf(cur[i][2 * e + 1], p.scale_log2, neg));
+                l += a;
+                l2 += b;
+                w[e] = pack2<DT>(a, b);
+            }
         };
 #pragma unroll
         for (int n = 0; n < AHEAD; n++)
@@ -334,36 +346,32 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
 #pragma unroll
         for (int n = 0; n < 2 * PER; n++) {
             const int i = n / PER, j = n % PER;
-            if (j < C::KS) {
+            if (kind == kFinal && j == 0)
+                weights(i, 0, 8);
+            if (j < QK) {
                 next[i] = mfma32<DT>(ring[n % (AHEAD + 1)], qf[j], j == 0 ? f32x16{} : next[i]);
             } else {
-                const int u = (j - C::KS) / C::DB, d = (j - C::KS) % C::DB;
+                const int u = (j - QK) / C::DB, d = (j - QK) % C::DB;
                 const s16x8 pf = __builtin_bit_cast(s16x8, (rl_u32x4{w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]}));
                 o[d] = mfma32<DT>(ring[n % (AHEAD + 1)], pf, o[d]);
             }
             if (n + AHEAD < 2 * PER)
                 fetch(n + AHEAD);
-            if (j < C::KS) {
-#pragma unroll
-                for (int e = 8 / C::KS * j; e < 8 / C::KS * (j + 1); e++) {
-                    const float a = __builtin_amdgcn_exp2f(fmaf(cur[i][2 * e], p.scale_log2, neg));
-                    const float b = __builtin_amdgcn_exp2f(fmaf(cur[i][2 * e + 1], p.scale_log2, neg));
-                    l += a;
-                    l2 += b;
-                    w[e] = pack2<DT>(a, b);
-                }
-            } else {
+            if (j < QK) {
+                weights(i, 8 / C::KS * j, 8 / C::KS * (j + 1));
+            } else if (kind != kFinal) {
                 constexpr int E = 16 / (2 * C::DB);
 #pragma unroll
-                for (int r = E * (j - C::KS); r < E * (j - C::KS + 1); r++) {
-                    if (masked)
+                for (int r = E * (j - QK); r < E * (j - QK + 1); r++) {
+                    if (kind == kMasked)
                         next[i][r] = hide(next[i][r], k_next + 32 * i, r);
                     top = fmaxf(top, next[i][r]);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        raise(top);
+        if (kind != kFinal)
+            raise(top);
     };
 
     // ---- the tiles -------------------------------------------------------------
@@ -394,36 +402,64 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
             raise(top);
         }
     }
-    // (Past a wave's last key the "next" scores are hidden whole, whatever the
-    // buffer holds.)
-    auto turn = [&](auto parity, auto masked, uint32_t s, f32x16 (&cur)[2], f32x16 (&next)[2]) {
-        const uint32_t t0 = (first + s) * BT;
+    auto meet = [&](auto whole, uint32_t s) {
         rl_wait_vmcnt<0>();
         rl_wait_lgkmcnt0();
         __builtin_amdgcn_s_barrier();  // K of step s + 1 and V of step s are there; nobody reads K of step s or V of s - 1
         asm volatile("" ::: "memory");
-        constexpr std::bool_constant<!decltype(masked)::value> whole{};
 #pragma unroll
         for (int i = 0; i < WOPS; i++)
             copy_k(whole, s + 2, i);
 #pragma unroll
         for (int i = 0; i < WOPS; i++)
             copy_v(whole, s + 1, i);
-        if (!decltype(masked)::value || t0 < w_most)
-            step(parity, masked, cur, next, t0 + BT);
     };
-    // the steps whose next scores every row of the wave sees whole and whose copies are of whole tiles, then the rest
     constexpr std::integral_constant<int, 0> even{};
     constexpr std::integral_constant<int, 1> uneven{};
+    constexpr std::integral_constant<int, kPlain> plain{};
+    constexpr std::integral_constant<int, kMasked> masked{};
+    constexpr std::integral_constant<int, kFinal> final{};
+    auto turn = [&](auto parity, auto kind, uint32_t s, f32x16 (&cur)[2], f32x16 (&next)[2]) {
+        meet(std::bool_constant<decltype(kind)::value == kPlain>{}, s);
+        step(parity, kind, cur, next, (first + s + 1) * BT);
+    };
+    // The steps, two by two: those whose next scores every row of the wave sees
+    // whole (and whose copies are of whole tiles), those whose next scores have
+    // some to hide, the wave's last one or two, and those of the other waves.
+    const uint32_t mine = w_most > first * BT ? (w_most + BT - 1) / BT - first : 0u;
     uint32_t s = 0;
-    for (; (uint64_t)(first + s + 3) * BT <= w_least && (uint64_t)(first + s + 4) * BT <= lk; s += 2) {
-        turn(even, std::false_type{}, s, sa, sb);
-        turn(uneven, std::false_type{}, s + 1, sb, sa);
+    for (; (uint64_t)(first + s + 3) * BT <= w_least && (uint64_t)min(first + s + 4, last) * BT <= lk; s += 2) {
+        turn(even, plain, s, sa, sb);
+        turn(uneven, plain, s + 1, sb, sa);
     }
-    for (; s < steps; s += 2) {
-        turn(even, std::true_type{}, s, sa, sb);
-        if (s + 1 < steps)
-            turn(uneven, std::true_type{}, s + 1, sb, sa);
+    if constexpr (SPLIT) {
+        // (without the steps that have no next scores: with them the compiler
+        // spills the shares' kernel, 24.4 to 34.3 us at 16 queries behind 6,000 keys)
+        auto turn_if = [&](auto parity, uint32_t s, f32x16 (&cur)[2], f32x16 (&next)[2]) {
+            meet(maybe, s);
+            if ((first + s) * BT < w_most)
+                step(parity, masked, cur, next, (first + s + 1) * BT);
+        };
+        for (; s < steps; s += 2) {
+            turn_if(even, s, sa, sb);
+            if (s + 1 < steps)
+                turn_if(uneven, s + 1, sb, sa);
+        }
+    } else {
+        for (; s + 2 < mine; s += 2) {
+            turn(even, masked, s, sa, sb);
+            turn(uneven, masked, s + 1, sb, sa);
+        }
+        if (s + 2 == mine) {
+            turn(even, masked, s, sa, sb);
+            turn(uneven, final, s + 1, sb, sa);
+            s += 2;
+        } else if (s + 1 == mine) {
+            turn(even, final, s, sa, sb);
+            s += 1;
+        }
+        for (; s < steps; s++)
+            meet(maybe, s);
     }
     rl_wait_vmcnt<0>();
     const float L = half_sum(l + l2);
