@@ -44,7 +44,6 @@ namespace {
 constexpr int kUnit = 32;           // tokens per unit
 constexpr uint32_t kRowCost = 8;    // units that turning to a row is worth
 
-
 struct Kv8Params {
     const uint8_t *arena;
     uint64_t block_bytes;
@@ -677,7 +676,8 @@ int validate(const rl_attn_decode_args_t *a, const char *who)
         rl_set_error("%s: grid_waves %u (only 0, the library's own split)", who, a->grid_waves);
         return -1;
     }
-    if ((uint64_t)a->batch * a->kv_heads * (((uint64_t)a->max_ctx + kUnit - 1) / kUnit) >= (1ull << 32)) {
+    // (the even kernel counts a row's units and its cost in 32 bits)
+    if ((uint64_t)a->batch * a->kv_heads * (((uint64_t)a->max_ctx + kUnit - 1) / kUnit + kRowCost) >= (1ull << 32)) {
         rl_set_error("%s: batch %u x kv_heads %u of max_ctx %u exceeds 2^32 units of %d tokens", who, a->batch,
                      a->kv_heads, a->max_ctx, kUnit);
         return -1;

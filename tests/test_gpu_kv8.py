@@ -203,6 +203,32 @@ def test_decode_splits(rl, gpu, batch, max_ctx, lens):
     assert np.array_equal(again[1].view(np.uint32), out32.view(np.uint32))
 
 
+@pytest.mark.parametrize("batch, kvh, group, t, d, dtype, max_ctx, lens", [
+    (100, 2, 16, 16, 128, "bf16", 900, (1, 260)),   # one row per compute unit, eight waves, sixteen heads
+    (160, 1, 1, 32, 64, "fp16", 800, (0, 800)),     # the same, small heads
+    (64, 2, 4, 16, 128, "bf16", 4096, (0, 200)),    # even shares, most rows short
+    (130, 1, 8, 32, 128, "fp16", 4100, (0, 90)),    # even shares, three groups of 64 rollouts
+    (7, 3, 2, 16, 64, "bf16", 200000, (3000, 9000)),  # even shares, rows in many pieces
+])
+def test_decode_kernels(rl, gpu, batch, kvh, group, t, d, dtype, max_ctx, lens):
+    """Every way the rows are shared out, with empty rows first, last and between."""
+    rng = np.random.default_rng(batch)
+    ctx = rng.integers(lens[0], lens[1] + 1, batch)
+    ctx[rng.random(batch) < 0.15] = 0
+    ctx[[0, -1]] = 0, 0 if batch % 2 else lens[1]
+    ctx = ctx.tolist()
+    arena, table, q = decode_case(rng, ctx, kvh, group, t, d, dtype, stride=-(-max_ctx // t))
+    out16, out32 = k8.run_decode(rl, arena, table, ctx, q, dtype, max_ctx)
+    for b in range(batch):
+        assert ctx[b] or not out32[b].any()
+    check(arena, table, ctx, q, out16, out32, dtype)
+    again = k8.run_decode(rl, arena, table, ctx, q, dtype, max_ctx, graph=2)
+    assert np.array_equal(again[1].view(np.uint32), out32.view(np.uint32))
+    # no tokens at all
+    out16, out32 = k8.run_decode(rl, arena, table, [0] * batch, q, dtype, max_ctx)
+    assert not out32.any() and not out16.any()
+
+
 def test_decode_bad_rows(rl, gpu):
     """A context past max_ctx and a block past the arena give NaN rows; the others keep their bits. NaN among a row's own
     tokens reaches only the outputs that see it."""

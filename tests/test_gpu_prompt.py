@@ -79,6 +79,29 @@ def test_pieces(rl, gpu, d, qh, kvh, dtype):
     assert not out[qs[3]:qs[3] + 3].any() and not out[qs[4]:qs[5]].any()
 
 
+@pytest.mark.parametrize("d, kvh, dtype", [(128, 1, "bf16"), (64, 3, "fp16")])
+def test_tile_counts(rl, gpu, d, kvh, dtype):
+    """Sequences of two to eight tiles, whole and not, and equal ones: every order of the kinds of steps."""
+    rng = np.random.default_rng(d)
+    lens = [128, 192, 193, 256, 319, 320, 385, 448, 192, 512]
+    qs = starts_of(lens)
+    q, k, v = inputs(rng, qs[-1], qs[-1], 2 * kvh, kvh, d, dtype)
+    out = run(rl, q, k, v, qs, kvh, dtype)
+    compare(out.reshape(q.shape), q, k, v, qs, qs, kvh, dtype)
+    assert np.array_equal(run(rl, q, k, v, qs, kvh, dtype, graph=3), out)
+
+
+def test_many_sequences(rl, gpu):
+    """More sequences than are put in order, most of one or two tokens, and a key group that no XCD count divides."""
+    rng = np.random.default_rng(70)
+    lens = rng.integers(0, 4, 90).tolist()
+    lens[33], lens[88] = 140, 77
+    qs = starts_of(lens)
+    q, k, v = inputs(rng, qs[-1], qs[-1], 9, 3, 64, "bf16")
+    out = run(rl, q, k, v, qs, 3, "bf16")
+    compare(out.reshape(q.shape), q, k, v, qs, qs, 3, "bf16")
+
+
 @pytest.mark.parametrize("n, kvh", [(1500, 2), (2100, 1)])
 def test_long(rl, gpu, n, kvh):
     rng = np.random.default_rng(n)
@@ -136,6 +159,26 @@ def test_what_is_not_seen_has_no_part(rl, gpu, d):
     assert np.isnan(f[70:100, :2, 3]).all() and same[70:100, :2][..., np.arange(d) != 3].all()
     assert np.isposinf(f[90:100, 2:, 5]).all() and same[90:100, 2:][..., np.arange(d) != 5].all() and same[70:90, 2:].all()
     assert np.isnan(f[180:249, 2:]).all() and np.isnan(f[249]).all()
+
+
+def test_shares_and_what_is_not_seen(rl, gpu):
+    """The same where workgroups share a row's keys: the last queries of a long sequence, a value that is no number among
+    the keys that only the last one sees, and one that all see."""
+    rng = np.random.default_rng(18)
+    nq, nk = 5, 3000
+    q, k, v = inputs(rng, nq, nk, 4, 1, 128, "bf16")
+    clean = k8.floats(run(rl, q, k, v, [0, nq], 1, "bf16", kv_starts=[0, nk]).reshape(q.shape), "bf16")
+    bad = k8.floats(v, "bf16")
+    bad[nk - 1, 0, 7] = np.nan
+    bad[nk - 2, 0, 8] = -np.inf
+    bad[1000, 0, 9] = np.inf
+    f = k8.floats(run(rl, q, k, k8.bits(bad, "bf16"), [0, nq], 1, "bf16", kv_starts=[0, nk]).reshape(q.shape), "bf16")
+    tol = 3 * k8.HALF_STEP["bf16"] * np.abs(clean) + 2 * k8.HALF_STEP["bf16"]
+    same = np.abs(f - clean) <= tol
+    assert np.isposinf(f[:, :, 9]).all() and np.isnan(f[4, :, 7]).all() and np.isneginf(f[3:, :, 8]).all()
+    seen = np.ones(f.shape, bool)
+    seen[:, :, 9] = seen[4, :, 7] = seen[3:, :, 8] = False
+    assert same[seen].all()
 
 
 def test_strides_and_bounds(rl, gpu):

@@ -86,6 +86,8 @@ def test_append_refusals(rl, kw, words):
     (dict(q_heads=12), "kv_heads"), (dict(q_heads=136), "kv_heads"), (dict(kv_heads=0), "kv_heads"),
     (dict(q_heads=0), "kv_heads"), (dict(batch=0), "batch"), (dict(batch=65536), "batch"),
     (dict(arena_bytes=100), "no block"), (dict(grid_waves=8), "grid_waves"), (dict(max_ctx=65), "table_stride"),
+    (dict(batch=65535, kv_heads=256, q_heads=256, max_ctx=8000, table_stride=500), "units"),
+    (dict(batch=65535, kv_heads=257, q_heads=257), "batch"),
     (dict(arena_base=P + 64 + 8), "aligned"), (dict(q=P + 2), "aligned")])
 def test_decode_refusals(rl, kw, words):
     kw = {k: v(rl) if callable(v) else v for k, v in kw.items()}
