@@ -668,8 +668,12 @@ int validate(const rl_attn_decode_args_t *a, const char *who)
         rl_set_error("%s: arena of %llu bytes holds no block", who, (unsigned long long)a->arena_bytes);
         return -1;
     }
-    if (a->batch == 0 || a->batch > 65535 || a->kv_heads > 65535 || (uint64_t)a->batch * a->kv_heads > (1u << 24)) {
-        rl_set_error("%s: batch %u / kv_heads %u out of range", who, a->batch, a->kv_heads);
+    // (a launch holds less than 2^32 work-items: the merge 256 for each 256 output elements of a row)
+    const uint64_t elements = (uint64_t)(a->q_heads / a->kv_heads) * a->layout.head_dim;
+    if (a->batch == 0 || a->batch > 65535 || a->kv_heads > 65535 ||
+        (uint64_t)a->batch * a->kv_heads * ((elements + 255) / 256) >= (1u << 24)) {
+        rl_set_error("%s: batch %u / kv_heads %u out of range (%llu output elements per row)", who, a->batch,
+                     a->kv_heads, (unsigned long long)elements);
         return -1;
     }
     if (a->grid_waves != 0) {

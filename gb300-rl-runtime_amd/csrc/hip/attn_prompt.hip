@@ -54,7 +54,7 @@ struct PromptParams {
     uint16_t *out;
     uint64_t q_stride, k_stride, v_stride, out_stride;  // elements between tokens
     const uint32_t *q_starts, *kv_starts;
-    uint32_t q_tokens, kv_tokens;
+    uint32_t q_tokens, kv_tokens, max_q;
     uint32_t kv_heads, group;
     uint32_t pairs;   // sequences x KV heads
     uint32_t tiles;   // row blocks of the longest sequence
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     const uint32_t qs = rl_sload(p.q_starts + seq), qe = min(rl_sload(p.q_starts + seq + 1), p.q_tokens);
     const uint32_t ks = rl_sload(p.kv_starts + seq), ke = min(rl_sload(p.kv_starts + seq + 1), p.kv_tokens);
     const uint32_t lq = qe > qs ? qe - qs : 0u, lk = ke > ks ? ke - ks : 0u;
-    const uint64_t rows = (uint64_t)lq * p.group;
+    const uint64_t rows = (uint64_t)min(lq, p.max_q) * p.group;
     const uint64_t wg_row = (uint64_t)tile * ROWS;
     if (wg_row >= rows)
         return;
@@ -516,11 +516,13 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     // row whose sum is no number is right as it is: NaN.)
     uint64_t again = __builtin_amdgcn_ballot_w64(odd != 0.f && L == L && my_row < rows);
     again = (again | again >> 32) & 0xFFFFFFFFu;
+    if (again)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (other lanes' stores to the same places came first)
     while (again) {
         const int r = __builtin_ctzll(again);
         again &= again - 1;
         const uint32_t tok = rl_readlane(my_tok, r), head = rl_readlane(my_head, r), n = rl_readlane(my_seen, r);
-        const float mr = __uint_as_float(rl_readlane(__float_as_uint(m), r));
+        const float mr = __uint_as_float(rl_readlane(__float_as_uint(m), r)), neg = mr == -INFINITY ? 0.f : -mr;
         const float lr = __uint_as_float(rl_readlane(__float_as_uint(L), r));
         constexpr int E = D / 64;  // dims per lane
         const uint16_t *q = p.q + (uint64_t)(qs + tok) * p.q_stride + (uint64_t)head * D + lane * E;
@@ -540,7 +542,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
 #pragma unroll
             for (int x = 1; x < 64; x *= 2)
                 s += __shfl_xor(s, x);
-            const float w = __builtin_amdgcn_exp2f(fmaf(s, p.scale_log2, -mr));
+            const float w = __builtin_amdgcn_exp2f(fmaf(s, p.scale_log2, neg));
 #pragma unroll
             for (int e = 0; e < E; e++)
                 acc[e] = fmaf(w, from16<DT>(vr[e]), acc[e]);
@@ -575,7 +577,7 @@ __global__ __launch_bounds__(NW * 64) void attn_prompt_merge_kernel(PromptParams
     const uint32_t qs = rl_sload(p.q_starts + seq), qe = min(rl_sload(p.q_starts + seq + 1), p.q_tokens);
     const uint32_t ks = rl_sload(p.kv_starts + seq), ke = min(rl_sload(p.kv_starts + seq + 1), p.kv_tokens);
     const uint32_t lq = qe > qs ? qe - qs : 0u, lk = ke > ks ? ke - ks : 0u;
-    const uint64_t rows = (uint64_t)lq * p.group;
+    const uint64_t rows = (uint64_t)min(lq, p.max_q) * p.group;
     const uint64_t wg_row = (uint64_t)tile * ROWS, row = wg_row + wave * 32 + (lane & 31);
     if (wg_row >= rows)
         return;
@@ -633,16 +635,12 @@ PromptPlan plan_of(const rl_attn_prompt_args_t *a)
 template <int D, int DT>
 int launch(const PromptParams &p)
 {
-    const uint64_t grid = (uint64_t)p.pairs * p.tiles * p.split;
-    if (grid > 0x7FFFFFFFull / 4) {
-        rl_set_error("rl_hip_attn_prompt: %llu workgroups", (unsigned long long)grid);
-        return -1;
-    }
+    const uint32_t grid = p.pairs * p.tiles * p.split;
     if (p.split == 1) {
-        hipLaunchKernelGGL((attn_prompt_kernel<D, DT, false>), dim3((uint32_t)grid), dim3(NW * 64), 0, rl_stream(), p);
+        hipLaunchKernelGGL((attn_prompt_kernel<D, DT, false>), dim3(grid), dim3(NW * 64), 0, rl_stream(), p);
         return rl_check_launch("attn_prompt_kernel launch");
     }
-    hipLaunchKernelGGL((attn_prompt_kernel<D, DT, true>), dim3((uint32_t)grid), dim3(NW * 64), 0, rl_stream(), p);
+    hipLaunchKernelGGL((attn_prompt_kernel<D, DT, true>), dim3(grid), dim3(NW * 64), 0, rl_stream(), p);
     if (rl_check_launch("attn_prompt_kernel launch"))
         return -1;
     hipLaunchKernelGGL((attn_prompt_merge_kernel<D, DT>), dim3(p.pairs * p.tiles * PCfg<D>::DB), dim3(NW * 64), 0,
@@ -676,6 +674,13 @@ int validate(const rl_attn_prompt_args_t *a, const char *who)
     if ((uint64_t)a->max_q * group >= (1ull << 31) || a->max_kv >= (1u << 31)) {
         rl_set_error("%s: max_q %u x %llu heads per KV head / max_kv %u of 2^31 and above", who, a->max_q,
                      (unsigned long long)group, a->max_kv);
+        return -1;
+    }
+    // (a launch holds less than 2^32 work-items)
+    const uint64_t blocks = (uint64_t)a->seqs * a->kv_heads * ((a->max_q * group + ROWS - 1) / ROWS);
+    if (blocks >= (1u << 24)) {
+        rl_set_error("%s: %llu blocks of %u rows (%u sequences of up to %u queries, %u KV heads; less than 2^24)", who,
+                     (unsigned long long)blocks, ROWS, a->seqs, a->max_q, a->kv_heads);
         return -1;
     }
     if (!(a->scale >= 0.f) || std::isinf(a->scale)) {
@@ -737,6 +742,7 @@ extern "C" int rl_hip_attn_prompt(const rl_attn_prompt_args_t *a)
     p.kv_starts = a->kv_starts ? a->kv_starts : a->q_starts;
     p.q_tokens = a->q_tokens;
     p.kv_tokens = a->kv_tokens;
+    p.max_q = a->max_q;
     p.kv_heads = a->kv_heads;
     p.group = a->q_heads / a->kv_heads;
     const float scale = a->scale != 0.f ? a->scale : 1.0f / sqrtf((float)a->head_dim);

@@ -19,6 +19,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "attn_core.h"
 #include "kv8_core.h"
 #include "rl_hip.h"
@@ -37,7 +39,7 @@ struct Append8Params {
     uint32_t table_stride;
     uint32_t kv_heads;
     uint32_t touched;   // blocks of a row that max_new tokens may reach
-    uint64_t items;     // batch * touched * kv_heads
+    uint32_t items;     // batch * touched * kv_heads
     const uint32_t *positions;
     const uint32_t *starts;  // NULL: one token per row
     uint32_t tokens;
@@ -66,12 +68,11 @@ __global__ __launch_bounds__(kWaves * 64) void kv8_append_kernel(Append8Params p
     constexpr int RPP = 64 / LPR;          // tokens per pass
     constexpr int PASSES = TPB / RPP;
     const int lane = threadIdx.x & 63;
-    const uint64_t item = (uint64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t item = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (item >= p.items)
         return;
-    const uint32_t g = (uint32_t)(item % p.kv_heads);
-    const uint64_t bj = item / p.kv_heads;
-    const uint32_t b = (uint32_t)(bj / p.touched), j = (uint32_t)(bj % p.touched);
+    const uint32_t g = item % p.kv_heads, bj = item / p.kv_heads;
+    const uint32_t b = bj / p.touched, j = bj % p.touched;
 
     const uint32_t pos = rl_sload(p.positions + b);
     uint32_t first = b, n = b < p.tokens ? 1u : 0u;
@@ -182,16 +183,20 @@ __global__ __launch_bounds__(kWaves * 64) void kv8_append_kernel(Append8Params p
 template <int D, int TPB>
 int launch(const Append8Params &p, uint32_t dtype)
 {
-    const uint64_t grid = (p.items + kWaves - 1) / kWaves;
-    if (grid > 0x7FFFFFFFull) {
-        rl_set_error("rl_hip_kv8_append: %llu workgroups", (unsigned long long)grid);
-        return -1;
-    }
+    const uint32_t grid = (p.items + kWaves - 1) / kWaves;
     if (dtype == RL_DTYPE_BF16)
-        hipLaunchKernelGGL((kv8_append_kernel<D, TPB, 0>), dim3((uint32_t)grid), dim3(kWaves * 64), 0, rl_stream(), p);
+        hipLaunchKernelGGL((kv8_append_kernel<D, TPB, 0>), dim3(grid), dim3(kWaves * 64), 0, rl_stream(), p);
     else
-        hipLaunchKernelGGL((kv8_append_kernel<D, TPB, 1>), dim3((uint32_t)grid), dim3(kWaves * 64), 0, rl_stream(), p);
+        hipLaunchKernelGGL((kv8_append_kernel<D, TPB, 1>), dim3(grid), dim3(kWaves * 64), 0, rl_stream(), p);
     return rl_check_launch("kv8_append_kernel launch");
+}
+
+// Blocks of a row that max_new tokens may reach: the worst first position is a
+// block's last slot, and the table has no more.
+uint64_t touched_of(const rl_kv8_append_args_t *a)
+{
+    const uint64_t tpb = a->layout.token_count;
+    return std::min<uint64_t>(((uint64_t)a->max_new + tpb - 2) / tpb + 1, a->table_stride);
 }
 
 int validate(const rl_kv8_append_args_t *a)
@@ -216,6 +221,12 @@ int validate(const rl_kv8_append_args_t *a)
     }
     if (a->max_new == 0 || (!a->starts && a->max_new != 1)) {
         rl_set_error("%s: max_new %u (1 without starts, at least 1 with them)", who, a->max_new);
+        return -1;
+    }
+    // (a launch holds less than 2^32 work-items, 64 for each of these)
+    if ((uint64_t)a->batch * a->kv_heads * touched_of(a) > (1u << 25)) {
+        rl_set_error("%s: batch %u x kv_heads %u x the blocks of max_new %u tokens exceed 2^25", who, a->batch,
+                     a->kv_heads, a->max_new);
         return -1;
     }
     if (!a->starts && a->tokens != a->batch) {
@@ -255,12 +266,10 @@ extern "C" int rl_hip_kv8_append(const rl_kv8_append_args_t *a)
     p.table = a->block_table;
     p.table_stride = a->table_stride;
     p.kv_heads = a->kv_heads;
-    // the worst first position is a block's last slot; never more blocks than the table has
-    const uint64_t touched = ((uint64_t)a->max_new + tpb - 2) / tpb + 1;
-    p.touched = (uint32_t)(touched < a->table_stride ? touched : a->table_stride);
+    p.touched = (uint32_t)touched_of(a);
     if (p.touched == 0)
         return 0;  // a table without entries: every position lies past it
-    p.items = (uint64_t)a->batch * p.touched * a->kv_heads;
+    p.items = a->batch * p.touched * a->kv_heads;
     p.positions = a->positions;
     p.starts = a->starts;
     p.tokens = a->tokens;

@@ -153,7 +153,8 @@ typedef struct {
     uint32_t seqs;               /* 1 .. 65,535 */
     uint32_t q_tokens;           /* rows of q and out */
     uint32_t kv_tokens;          /* rows of k and v */
-    uint32_t max_q;              /* upper bound of the sequences' queries; later ones get no output */
+    uint32_t max_q;              /* upper bound of the sequences' queries; later ones get no output. */
+                                 /* seqs * kv_heads * ceil(max_q * q_heads / kv_heads / 128) < 2^24 */
     uint32_t max_kv;             /* upper bound of their keys (it only guides the split of the work) */
     uint32_t q_heads;
     uint32_t kv_heads;           /* divides q_heads */
@@ -186,15 +187,19 @@ int rl_hip_attn_prompt(const rl_attn_prompt_args_t *args);
  * (shared) block of the arena instead, as in rl_hip_kv_append. Slots behind
  * the last new token keep their bytes and mean nothing. Positions past the
  * block table and blocks past arena_bytes are skipped. Two rows of one call
- * must not write the same block.
+ * must not write the same block, and none may write one that another's cow_src
+ * names: its scale could change under the copy. batch * kv_heads * the blocks
+ * that max_new tokens reach (at most table_stride) is up to 2^25.
  *
  * rl_hip_attn_decode_kv8 is rl_hip_attn_decode over such an arena, with its
  * arguments and rules: one query token per row, zeros for a context of 0, NaN
  * for a row whose context exceeds max_ctx or whose table names a block past
  * arena_bytes. The products are those of the e4m3 values times their scales
  * with fp32 sums (within 1e-4 of fp64). Any q_heads / kv_heads from 1 to 16;
- * grid_waves must be 0. A row's result depends on its own inputs and on
- * batch, kv_heads and max_ctx, not on the other rows. */
+ * grid_waves must be 0, and batch * kv_heads * ceil(q_heads / kv_heads *
+ * head_dim / 256) below 2^24. The same call gives the same bits; where long
+ * contexts are cut in even shares over the whole batch, the order of a row's
+ * sums depends on the other rows' lengths too. */
 typedef struct {
     void *arena_base;            /* device, 16-byte aligned */
     uint64_t arena_bytes;        /* blocks past it are never read or written */

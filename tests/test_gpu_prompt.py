@@ -203,6 +203,36 @@ def test_strides_and_bounds(rl, gpu):
     assert np.array_equal(few[10:43], out[10:43]) and np.array_equal(few[75:108], out[75:108])
 
 
+@pytest.mark.parametrize("max_q", [1, 33, 64])
+def test_queries_past_max_q(rl, gpu, max_q):
+    """A sequence's queries from max_q on get no output; the others are those without them."""
+    rng = np.random.default_rng(11)
+    lens, kvh = [100, 20, 65], 2
+    qs = starts_of(lens)
+    q, k, v = inputs(rng, qs[-1], qs[-1], 6, kvh, 128, "bf16")
+    cut = run(rl, q, k, v, qs, kvh, "bf16", max_q=max_q)
+    for a, n in zip(qs, lens):
+        m = min(n, max_q)
+        compare(cut[a:a + m].reshape(m, 6, 128), q[a:a + m], k[a:a + m], v[a:a + m], [0, m], [0, m], kvh, "bf16")
+        assert (cut[a + m:a + n] == 0x1234).all()
+
+
+def test_scores_without_weight(rl, gpu):
+    """A key whose score is minus infinity beside a value that is no number and that the row does not see, with the
+    keys shared by several workgroups: the row's other shares give its output."""
+    rng = np.random.default_rng(12)
+    nq, nk, finite = 2, 1500, 768  # three shares of eight tiles: the last one's scores are all minus infinity
+    q, k, v = inputs(rng, nq, nk, 1, 1, 64, "fp16")
+    fq, fk, fv = (k8.floats(x, "fp16") for x in (q, k, v))
+    fq[:, :, 0], fk[:finite, 0, 0], fk[finite:, 0, 0], fv[nk - 1, 0, 5] = 1.0, 0.0, -np.inf, np.nan
+    out = run(rl, *(k8.bits(x, "fp16") for x in (fq, fk, fv)), [0, nq], 1, "fp16", kv_starts=[0, nk])
+    out = k8.floats(out.reshape(q.shape), "fp16")
+    ref, mag = k8.attend(fq[:, 0], fk[:finite, 0], fv[:finite, 0], 1 / 8.0, [finite, finite])
+    tol = tolerance("fp16", ref, mag, fq[:, 0], fk[:finite, 0], 1 / 8.0, finite)
+    ok = np.abs(out[:, 0] - ref) <= tol
+    assert np.isnan(out[1, 0, 5]) and ok[0].all() and np.delete(ok[1], 5).all()
+
+
 def test_nothing_to_do(rl, gpu):
     a = rl.AttnPromptArgs(q=1 << 20, k=1 << 20, v=1 << 20, out=1 << 20, q_starts=1 << 20, seqs=1, q_tokens=0, kv_tokens=0,
                           max_q=0, max_kv=0, q_heads=8, kv_heads=2, head_dim=64, dtype=0, workspace=1 << 20,

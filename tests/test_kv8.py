@@ -72,6 +72,7 @@ L16 = ("layout", lambda rl: rl.KvLayoutDesc.paged(16, 128))
     (dict(k_new=None), "NULL"), (dict(v_new=None), "NULL"), (dict([L16]), "layout"), (dict(dtype=2), "dtype"),
     (dict(batch=0), "batch"), (dict(kv_heads=0), "kv_heads"), (dict(batch=65536, tokens=65536), "batch"),
     (dict(max_new=0), "max_new"), (dict(max_new=2), "max_new"), (dict(tokens=3), "tokens"),
+    (dict(batch=65535, starts=P, max_new=1 << 20, table_stride=1 << 16), "2^25"),
     (dict(arena_bytes=4223), "no block"), (dict(k_stride=1016), "stride"), (dict(v_stride=1028), "stride"),
     (dict(arena_base=P + 8), "aligned"), (dict(k_new=P + 2), "aligned"), (dict(v_new=P + 4), "aligned")])
 def test_append_refusals(rl, kw, words):
@@ -88,6 +89,7 @@ def test_append_refusals(rl, kw, words):
     (dict(arena_bytes=100), "no block"), (dict(grid_waves=8), "grid_waves"), (dict(max_ctx=65), "table_stride"),
     (dict(batch=65535, kv_heads=256, q_heads=256, max_ctx=8000, table_stride=500), "units"),
     (dict(batch=65535, kv_heads=257, q_heads=257), "batch"),
+    (dict(batch=65535, kv_heads=33, q_heads=528), "batch"),
     (dict(arena_base=P + 64 + 8), "aligned"), (dict(q=P + 2), "aligned")])
 def test_decode_refusals(rl, kw, words):
     kw = {k: v(rl) if callable(v) else v for k, v in kw.items()}
@@ -103,6 +105,7 @@ def test_decode_refusals(rl, kw, words):
     (dict(q_starts=None), "NULL"), (dict(head_dim=96), "head_dim"), (dict(q_heads=12), "kv_heads"),
     (dict(kv_heads=0), "kv_heads"), (dict(q_heads=0), "kv_heads"), (dict(dtype=2), "dtype"), (dict(seqs=0), "sequences"),
     (dict(seqs=65536), "sequences"), (dict(max_q=1 << 29), "max_q"), (dict(max_kv=1 << 31), "max_kv"),
+    (dict(seqs=65535, max_q=8192), "2^24"), (dict(seqs=65535, kv_heads=256, q_heads=256, max_q=129), "2^24"),
     (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
     (dict(q_stride=4088), "stride"), (dict(k_stride=1028), "stride"), (dict(v_stride=(1 << 24) + 8), "stride"),
     (dict(out_stride=100), "stride"), (dict(q=P + 8), "aligned"), (dict(k=P + 2), "aligned"), (dict(out=P + 4), "aligned")])
