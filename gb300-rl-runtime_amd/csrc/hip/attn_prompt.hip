@@ -5,12 +5,17 @@
 //
 // of a sequence with Lq queries and Lk >= Lq keys (the queries are its last
 // tokens). Bound: the matrix cores from some hundred tokens on, 4 head_dim
-// operations per head and visible pair; K and V come from L2.
+// operations per head and visible pair; K and V come from L2. Measured, bf16,
+// GQA 4, 8 KV heads, d128: 1 x 8,192 tokens 482-487 us, 1,130 TFLOP/s (372 with
+// zeros: the chip's power sets the clock), 64 x 512-1,024 477 us, 673 TFLOP/s (6.5
+// key tiles per row block, each with its own start and end), 1 x 517 13.3 us
+// (latency).
 //
 //  rows   a workgroup of NW waves takes 32 NW rows of one (sequence, KV head);
 //         row r is query token r / G, head r % G of the group, so that a
 //         group's heads share every K and V tile and a wave's rows span few
 //         tokens (little masked work on the diagonal).
+//         Eight waves per workgroup, or two groups of keys in one, were no faster.
 //  stage  64 tokens of K and V are copied to LDS with global_load_lds (16 B per
 //         lane), double-buffered, one barrier per tile. The 16-byte chunks of
 //         a row are permuted so that the operand reads below meet no bank
@@ -314,7 +319,9 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     // of their operands AHEAD instructions earlier and the vector work are laid
     // out here one by one: left to itself the compiler gathers each kind, and
     // then matrix cores and vector units take turns instead of working side by
-    // side.
+    // side. AHEAD: 2 is best, 3 costs 2%, 1 much more. The sum in plain adds: a
+    // dot product instruction does not run beside a matrix one (73-76 cycles
+    // per matrix instruction and its share of the weights, 46-49 with adds).
     auto step = [&](auto parity_, auto kind_, f32x16 (&cur)[2], f32x16 (&next)[2], uint32_t k_next) {
         constexpr int parity = decltype(parity_)::value;
         constexpr int kind = decltype(kind_)::value;
@@ -613,6 +620,11 @@ __global__ __launch_bounds__(NW * 64) void attn_prompt_merge_kernel(PromptParams
                                              pack2<DT>(o[4 * a + 2] * inv, o[4 * a + 3] * inv)};
 }
 
+// Few row blocks share their keys, in shares of eight tiles and more, as many as
+// compute units are left: 16 queries behind 6,000 keys 24.4 us against 80.4 of one
+// workgroup per row block, 300 behind 2,000 30.7 against 39.1. With 256 row
+// blocks and more it costs: pieces of four prompts behind 4,000 tokens 74 us,
+// 90 with every row block in two.
 struct PromptPlan {
     uint32_t tiles, pairs, split;
     size_t workspace;
@@ -753,6 +765,8 @@ extern "C" int rl_hip_attn_prompt(const rl_attn_prompt_args_t *a)
     p.split = pl.split;
     p.part = (float *)a->workspace;
     p.by_xcd = p.pairs % 8 == 0;
+    // (longest sequences first: 9 of 3-2,047 tokens, d64, 31.5 us, 36 in batch order; each
+    // workgroup ranks for itself, so not for long lists)
     p.ranked = p.seqs > 1 && p.seqs <= 64 && (uint64_t)p.pairs * p.tiles <= 4096;
     if (a->head_dim == 128)
         return a->dtype == RL_DTYPE_BF16 ? launch<128, 0>(p) : launch<128, 1>(p);
