@@ -54,6 +54,26 @@ constexpr uint32_t kShareTiles = 8;  // tiles per workgroup, at least, where sev
 constexpr int kPlain = 0, kMasked = 1, kFinal = 2;  // what a step's next scores are: all seen, some hidden, none
 constexpr float kSlack = 8.f;  // log2 of what a weight may exceed its reference by
 
+// Division of n < 2^31 by d: with 2^(shift - 1) < d <= 2^shift and mul the ceiling
+// of 2^(31 + shift) / d, floor(n mul / 2^(31 + shift)) is the quotient.
+struct Divisor {
+    uint32_t mul, shift;
+};
+
+Divisor divisor_of(uint32_t d)
+{
+    Divisor v = {0, 0};
+    while ((1ull << v.shift) < d)
+        v.shift++;
+    v.mul = (uint32_t)(((1ull << (31 + v.shift)) + d - 1) / d);
+    return v;
+}
+
+__device__ __forceinline__ uint32_t quotient(uint32_t n, const Divisor &v)
+{
+    return (uint32_t)((uint64_t)(n << 1) * v.mul >> 32) >> v.shift;
+}
+
 struct PromptParams {
     const uint16_t *q, *k, *v;
     uint16_t *out;
@@ -67,6 +87,7 @@ struct PromptParams {
     uint32_t ranked;  // the longest sequences first
     uint32_t seqs;
     uint32_t split;   // workgroups per row block, at most
+    Divisor by_group, by_pairs, by_heads, by_tiles;
     float scale_log2;
     float *part;      // [pairs x tiles][split][NW][PART] sums of split row blocks
 };
@@ -160,15 +181,16 @@ __device__ __forceinline__ void block_of(const PromptParams &p, uint32_t at, int
 {
     uint32_t pair;
     if (p.by_xcd) {
-        const uint32_t local = at / 8;
-        pair = at % 8 + 8 * (local / p.tiles);
-        tile = p.tiles - 1 - local % p.tiles;
+        const uint32_t local = at / 8, n = quotient(local, p.by_tiles);
+        pair = at % 8 + 8 * n;
+        tile = p.tiles - 1 - (local - n * p.tiles);
     } else {
-        pair = at % p.pairs;
-        tile = p.tiles - 1 - at / p.pairs;
+        const uint32_t n = quotient(at, p.by_pairs);
+        pair = at - n * p.pairs;
+        tile = p.tiles - 1 - n;
     }
-    seq = pair / p.kv_heads;
-    g = pair % p.kv_heads;
+    seq = quotient(pair, p.by_heads);
+    g = pair - seq * p.kv_heads;
     if (p.ranked)
         seq = seq_of_rank(p, seq, lane);
 }
@@ -190,14 +212,15 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     const uint32_t qs = rl_sload(p.q_starts + seq), qe = min(rl_sload(p.q_starts + seq + 1), p.q_tokens);
     const uint32_t ks = rl_sload(p.kv_starts + seq), ke = min(rl_sload(p.kv_starts + seq + 1), p.kv_tokens);
     const uint32_t lq = qe > qs ? qe - qs : 0u, lk = ke > ks ? ke - ks : 0u;
-    const uint64_t rows = (uint64_t)min(lq, p.max_q) * p.group;
-    const uint64_t wg_row = (uint64_t)tile * ROWS;
+    const uint32_t rows = min(lq, p.max_q) * p.group, wg_row = tile * ROWS;
     if (wg_row >= rows)
         return;
-    // keys that query token t sees: t + lk - lq + 1, not below 0
-    auto seen = [&](uint32_t t) { return (uint32_t)max<int64_t>((int64_t)t + lk - lq + 1, 0); };
-    const uint32_t wg_seen = seen((uint32_t)(min<uint64_t>(wg_row + ROWS, rows) - 1) / p.group);
-    const uint64_t w_row = wg_row + wave * 32;
+    // keys that query token t < lq sees: t + lk - lq + 1, not below 0
+    auto seen = [&](uint32_t t) { return (uint32_t)max((int32_t)(t - lq + 1) + (int32_t)lk, 0); };
+    const uint32_t wg_seen = seen(quotient(min(wg_row + ROWS, rows) - 1, p.by_group));
+    // the wave's rows: from head h0 of token tok0 on (those past the last row repeat it)
+    const uint32_t w_row = wg_row + wave * 32, w0 = min(w_row, rows - 1);
+    const uint32_t tok0 = quotient(w0, p.by_group), h0 = w0 - tok0 * p.group;
     // this workgroup's tiles of the keys: first .. first + steps - 1
     const uint32_t nt = (wg_seen + BT - 1) / BT;
     uint32_t first = 0, last = nt;
@@ -210,10 +233,10 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     }
     const uint32_t steps = last - first, most = (uint32_t)min<uint64_t>((uint64_t)last * BT, lk);
     const bool w_has = w_row < rows;
-    const uint32_t w_least = w_has ? min(most, seen((uint32_t)(w_row / p.group))) : 0u;
-    const uint32_t w_most = w_has ? min(most, seen((uint32_t)((min<uint64_t>(w_row + 32, rows) - 1) / p.group))) : 0u;
-    const uint64_t my_row = w_row + (lane & 31);
-    const uint32_t my_seen = min(most, seen((uint32_t)min<uint64_t>(my_row, rows - 1) / p.group));
+    const uint32_t w_least = w_has ? min(most, seen(tok0)) : 0u;
+    const uint32_t w_most = w_has ? min(most, seen(quotient(min(w_row + 32, rows) - 1, p.by_group))) : 0u;
+    const uint32_t my_x = h0 + min(w_row + ((uint32_t)lane & 31u), rows - 1) - w0, my_dt = quotient(my_x, p.by_group);
+    const uint32_t my_seen = min(most, seen(tok0 + my_dt));
 
     // ---- the copies --------------------------------------------------------------
     const uint16_t *kbase = p.k + (uint64_t)ks * p.k_stride + (uint64_t)g * D;
@@ -255,8 +278,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
 
     s16x8 qf[C::KS];
     {
-        const uint32_t r = (uint32_t)min<uint64_t>(my_row, rows - 1);
-        const uint16_t *q = p.q + (uint64_t)(qs + r / p.group) * p.q_stride + (uint64_t)(g * p.group + r % p.group) * D + 8 * hf;
+        const uint16_t *q = p.q + (uint64_t)(qs + tok0) * p.q_stride + (uint64_t)g * p.group * D;
+        q += my_dt * (uint32_t)p.q_stride + (my_x - my_dt * p.group) * D + 8 * hf;
 #pragma unroll
         for (int s = 0; s < C::KS; s++)
             qf[s] = *(const s16x8 *)(q + 16 * s);
@@ -395,11 +418,12 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
         if (first * BT < w_most) {
             float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                sa[i] = f32x16{};
+            for (int s = 0; s < C::KS; s++)
 #pragma unroll
-                for (int s = 0; s < C::KS; s++)
-                    sa[i] = mfma32<DT>(read_k(0, i, s), qf[s], sa[i]);
+                for (int i = 0; i < 2; i++)
+                    sa[i] = mfma32<DT>(read_k(0, i, s), qf[s], s == 0 ? f32x16{} : sa[i]);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     sa[i][r] = hide(sa[i][r], first * BT + 32 * i, r);
@@ -409,11 +433,13 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
             raise(top);
         }
     }
-    auto meet = [&](auto whole, uint32_t s) {
+    auto meet = [&](auto whole, uint32_t s, bool more) {
         rl_wait_vmcnt<0>();
         rl_wait_lgkmcnt0();
         __builtin_amdgcn_s_barrier();  // K of step s + 1 and V of step s are there; nobody reads K of step s or V of s - 1
         asm volatile("" ::: "memory");
+        if (!more)
+            return;
 #pragma unroll
         for (int i = 0; i < WOPS; i++)
             copy_k(whole, s + 2, i);
@@ -427,7 +453,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     constexpr std::integral_constant<int, kMasked> masked{};
     constexpr std::integral_constant<int, kFinal> final{};
     auto turn = [&](auto parity, auto kind, uint32_t s, f32x16 (&cur)[2], f32x16 (&next)[2]) {
-        meet(std::bool_constant<decltype(kind)::value == kPlain>{}, s);
+        meet(std::bool_constant<decltype(kind)::value == kPlain>{}, s, decltype(kind)::value != kFinal || s + 1 < steps);
         step(parity, kind, cur, next, (first + s + 1) * BT);
     };
     // The steps, two by two: those whose next scores every row of the wave sees
@@ -443,7 +469,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
         // (without the steps that have no next scores: with them the compiler
         // spills the shares' kernel, 24.4 to 34.3 us at 16 queries behind 6,000 keys)
         auto turn_if = [&](auto parity, uint32_t s, f32x16 (&cur)[2], f32x16 (&next)[2]) {
-            meet(maybe, s);
+            meet(maybe, s, s + 1 < steps);
             if ((first + s) * BT < w_most)
                 step(parity, masked, cur, next, (first + s + 1) * BT);
         };
@@ -466,15 +492,11 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
             s += 1;
         }
         for (; s < steps; s++)
-            meet(maybe, s);
+            meet(maybe, s, s + 1 < steps);
     }
     rl_wait_vmcnt<0>();
     const float L = half_sum(l + l2);
     // ---- the rows' outputs -------------------------------------------------------
-    uint32_t lane_row = (uint32_t)lane & 31u;
-    asm volatile("" : "+v"(lane_row));  // (token and head are found again here, not held through the loop)
-    const uint32_t out_row = (uint32_t)min<uint64_t>(w_row + lane_row, rows - 1);
-    const uint32_t my_tok = out_row / p.group, my_head = g * p.group + out_row % p.group;
     float odd = 0.f;
 #pragma unroll
     for (int d = 0; d < C::DB; d++)
@@ -495,8 +517,10 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     } else {
         // through LDS, so that a row leaves in whole lines
         const float inv = my_seen == 0 ? 0.f : 1.f / L;
-        __syncthreads();  // the tiles' room is free
+        if constexpr (SPLIT)
+            __syncthreads();  // (else nobody reads K in the last step, nor copies any)
         RL_LDS uint8_t *rows_lds = (RL_LDS uint8_t *)smem + wave * 32 * C::RB;
+        uint16_t *out = p.out + (uint64_t)(qs + tok0) * p.out_stride + (uint64_t)g * p.group * D;
         auto out_swz = [](uint32_t r) { return r & (C::NC - 1); };
 #pragma unroll
         for (int d = 0; d < C::DB; d++)
@@ -511,24 +535,25 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
 #pragma unroll
         for (int i = 0; i < C::NC / 2; i++) {
             const uint32_t r = i * (64 / C::NC) + (uint32_t)lane / C::NC, c = (uint32_t)lane % C::NC;
-            const uint32_t tok = (uint32_t)__shfl((int)my_tok, (int)r), head = (uint32_t)__shfl((int)my_head, (int)r);
             const rl_u32x4 w = *(RL_LDS const rl_u32x4 *)(rows_lds + r * C::RB + ((c ^ out_swz(r)) << 4));
+            const uint32_t dt = quotient(h0 + r, p.by_group), at = dt * (uint32_t)p.out_stride + (h0 + r - dt * p.group) * D;
             if (w_row + r < rows)
-                *(rl_u32x4 *)(p.out + (uint64_t)(qs + tok) * p.out_stride + (uint64_t)head * D + c * 8) = w;
+                *(rl_u32x4 *)(out + at + c * 8) = w;
         }
     }
     // A value of V that is no number spoils its whole 64-key tile in the matrix
     // product, also for the rows that do not see it (0 times NaN). Rows with
     // such an output are computed again, key by key, over what they see. (A
     // row whose sum is no number is right as it is: NaN.)
-    uint64_t again = __builtin_amdgcn_ballot_w64(odd != 0.f && L == L && my_row < rows);
+    uint64_t again = __builtin_amdgcn_ballot_w64(odd != 0.f && L == L && w_row + (lane & 31) < rows);
     again = (again | again >> 32) & 0xFFFFFFFFu;
     if (again)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (other lanes' stores to the same places came first)
     while (again) {
         const int r = __builtin_ctzll(again);
         again &= again - 1;
-        const uint32_t tok = rl_readlane(my_tok, r), head = rl_readlane(my_head, r), n = rl_readlane(my_seen, r);
+        const uint32_t dt = quotient(h0 + r, p.by_group), tok = tok0 + dt, head = g * p.group + h0 + r - dt * p.group;
+        const uint32_t n = rl_readlane(my_seen, r);
         const float mr = __uint_as_float(rl_readlane(__float_as_uint(m), r)), neg = mr == -INFINITY ? 0.f : -mr;
         const float lr = __uint_as_float(rl_readlane(__float_as_uint(L), r));
         constexpr int E = D / 64;  // dims per lane
@@ -584,12 +609,12 @@ __global__ __launch_bounds__(NW * 64) void attn_prompt_merge_kernel(PromptParams
     const uint32_t qs = rl_sload(p.q_starts + seq), qe = min(rl_sload(p.q_starts + seq + 1), p.q_tokens);
     const uint32_t ks = rl_sload(p.kv_starts + seq), ke = min(rl_sload(p.kv_starts + seq + 1), p.kv_tokens);
     const uint32_t lq = qe > qs ? qe - qs : 0u, lk = ke > ks ? ke - ks : 0u;
-    const uint64_t rows = (uint64_t)min(lq, p.max_q) * p.group;
-    const uint64_t wg_row = (uint64_t)tile * ROWS, row = wg_row + wave * 32 + (lane & 31);
+    const uint32_t rows = min(lq, p.max_q) * p.group;
+    const uint32_t wg_row = tile * ROWS, row = wg_row + wave * 32 + (lane & 31);
     if (wg_row >= rows)
         return;
-    const uint32_t last_tok = (uint32_t)(min<uint64_t>(wg_row + ROWS, rows) - 1) / p.group;
-    const uint32_t wg_seen = (uint32_t)max<int64_t>((int64_t)last_tok + lk - lq + 1, 0);
+    const uint32_t last_tok = quotient(min(wg_row + ROWS, rows) - 1, p.by_group);
+    const uint32_t wg_seen = (uint32_t)max((int32_t)(last_tok - lq + 1) + (int32_t)lk, 0);
     const uint32_t n = shares_of(p, (wg_seen + BT - 1) / BT);
     if (n < 2 || row >= rows)
         return;
@@ -610,8 +635,8 @@ __global__ __launch_bounds__(NW * 64) void attn_prompt_merge_kernel(PromptParams
         for (int r = 0; r < 16; r++)
             o[r] = fmaf(x[(16 * d + r) * 64], f, o[r]);
     }
-    const uint32_t tok = (uint32_t)row / p.group, head = g * p.group + (uint32_t)row % p.group;
-    const bool none = (int64_t)tok + lk - lq + 1 <= 0;
+    const uint32_t tok = quotient(row, p.by_group), head = g * p.group + row - tok * p.group;
+    const bool none = (int32_t)(tok - lq + 1) + (int32_t)lk <= 0;
     const float inv = none ? 0.f : 1.f / L;
     uint16_t *dst = p.out + (uint64_t)(qs + tok) * p.out_stride + (uint64_t)head * D + 32 * d + 4 * (lane >> 5);
 #pragma unroll
@@ -686,6 +711,10 @@ int validate(const rl_attn_prompt_args_t *a, const char *who)
     if ((uint64_t)a->max_q * group >= (1ull << 31) || a->max_kv >= (1u << 31)) {
         rl_set_error("%s: max_q %u x %llu heads per KV head / max_kv %u of 2^31 and above", who, a->max_q,
                      (unsigned long long)group, a->max_kv);
+        return -1;
+    }
+    if (a->q_tokens >= (1u << 31) || a->kv_tokens >= (1u << 31)) {
+        rl_set_error("%s: q_tokens %u / kv_tokens %u of 2^31 and above", who, a->q_tokens, a->kv_tokens);
         return -1;
     }
     // (a launch holds less than 2^32 work-items)
@@ -763,6 +792,10 @@ extern "C" int rl_hip_attn_prompt(const rl_attn_prompt_args_t *a)
     p.tiles = pl.tiles;
     p.pairs = pl.pairs;
     p.split = pl.split;
+    p.by_group = divisor_of(p.group);
+    p.by_pairs = divisor_of(p.pairs);
+    p.by_heads = divisor_of(p.kv_heads);
+    p.by_tiles = divisor_of(p.tiles);
     p.part = (float *)a->workspace;
     p.by_xcd = p.pairs % 8 == 0;
     // (longest sequences first: 9 of 3-2,047 tokens, d64, 31.5 us, 36 in batch order; each

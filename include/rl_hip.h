@@ -151,8 +151,8 @@ typedef struct {
     const uint32_t *q_starts;    /* device [seqs + 1], not decreasing */
     const uint32_t *kv_starts;   /* device [seqs + 1] or NULL: q_starts */
     uint32_t seqs;               /* 1 .. 65,535 */
-    uint32_t q_tokens;           /* rows of q and out */
-    uint32_t kv_tokens;          /* rows of k and v */
+    uint32_t q_tokens;           /* rows of q and out; below 2^31 */
+    uint32_t kv_tokens;          /* rows of k and v; below 2^31 */
     uint32_t max_q;              /* upper bound of the sequences' queries; later ones get no output. */
                                  /* seqs * kv_heads * ceil(max_q * q_heads / kv_heads / 128) < 2^24 */
     uint32_t max_kv;             /* upper bound of their keys (it only guides the split of the work) */

@@ -105,6 +105,7 @@ def test_decode_refusals(rl, kw, words):
     (dict(q_starts=None), "NULL"), (dict(head_dim=96), "head_dim"), (dict(q_heads=12), "kv_heads"),
     (dict(kv_heads=0), "kv_heads"), (dict(q_heads=0), "kv_heads"), (dict(dtype=2), "dtype"), (dict(seqs=0), "sequences"),
     (dict(seqs=65536), "sequences"), (dict(max_q=1 << 29), "max_q"), (dict(max_kv=1 << 31), "max_kv"),
+    (dict(q_tokens=1 << 31), "q_tokens"), (dict(kv_tokens=1 << 31), "kv_tokens"),
     (dict(seqs=65535, max_q=8192), "2^24"), (dict(seqs=65535, kv_heads=256, q_heads=256, max_q=129), "2^24"),
     (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
     (dict(q_stride=4088), "stride"), (dict(k_stride=1028), "stride"), (dict(v_stride=(1 << 24) + 8), "stride"),
