@@ -515,31 +515,28 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
         part[C::DB * 16 * 64 + lane] = m;
         part[(C::DB * 16 + 1) * 64 + lane] = L;
     } else {
-        // through LDS, so that a row leaves in whole lines
         const float inv = my_seen == 0 ? 0.f : 1.f / L;
-        if constexpr (SPLIT)
-            __syncthreads();  // (else nobody reads K in the last step, nor copies any)
-        RL_LDS uint8_t *rows_lds = (RL_LDS uint8_t *)smem + wave * 32 * C::RB;
         uint16_t *out = p.out + (uint64_t)(qs + tok0) * p.out_stride + (uint64_t)g * p.group * D;
-        auto out_swz = [](uint32_t r) { return r & (C::NC - 1); };
+        const uint32_t r = (uint32_t)lane & 31u, dt = quotient(h0 + r, p.by_group);
+        const uint32_t at = dt * (uint32_t)p.out_stride + (h0 + r - dt * p.group) * D + 8 * hf;
+        const bool has = w_row + r < rows;
 #pragma unroll
         for (int d = 0; d < C::DB; d++)
 #pragma unroll
-            for (int a = 0; a < 4; a++) {
-                const uint32_t r = (uint32_t)lane & 31u;
-                const rl_u32x2 w = {pack2<DT>(o[d][4 * a] * inv, o[d][4 * a + 1] * inv),
-                                    pack2<DT>(o[d][4 * a + 2] * inv, o[d][4 * a + 3] * inv)};
-                *(RL_LDS rl_u32x2 *)(rows_lds + r * C::RB + (((4u * d + a) ^ out_swz(r)) << 4) + 8 * hf) = w;
-            }
-        rl_wave_lds_fence();
+            for (int a = 0; a < 4; a += 2) {
+                // lanes l and l + 32 hold four dims each of both 8-dim chunks: each takes a whole one
+                rl_u32x4 w;
 #pragma unroll
-        for (int i = 0; i < C::NC / 2; i++) {
-            const uint32_t r = i * (64 / C::NC) + (uint32_t)lane / C::NC, c = (uint32_t)lane % C::NC;
-            const rl_u32x4 w = *(RL_LDS const rl_u32x4 *)(rows_lds + r * C::RB + ((c ^ out_swz(r)) << 4));
-            const uint32_t dt = quotient(h0 + r, p.by_group), at = dt * (uint32_t)p.out_stride + (h0 + r - dt * p.group) * D;
-            if (w_row + r < rows)
-                *(rl_u32x4 *)(out + at + c * 8) = w;
-        }
+                for (int e = 0; e < 2; e++) {
+                    const uint32_t x = pack2<DT>(o[d][4 * a + 2 * e] * inv, o[d][4 * a + 2 * e + 1] * inv);
+                    const uint32_t y = pack2<DT>(o[d][4 * a + 4 + 2 * e] * inv, o[d][4 * a + 5 + 2 * e] * inv);
+                    const auto h = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+                    w[e] = h[0];
+                    w[2 + e] = h[1];
+                }
+                if (has)
+                    *(rl_u32x4 *)(out + at + 32 * d + 8 * a) = w;
+            }
     }
     // A value of V that is no number spoils its whole 64-key tile in the matrix
     // product, also for the rows that do not see it (0 times NaN). Rows with
