@@ -376,6 +376,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
 #pragma unroll
         for (int n = 0; n < 2 * PER; n++) {
             const int i = n / PER, j = n % PER;
+            if (kind == kFinal && n == PER && k_next - 32 >= w_most)
+                break;  // (no row of the wave sees the tile's second half)
             if (kind == kFinal && j == 0)
                 weights(i, 0, 8);
             if (j < QK) {
