@@ -6,16 +6,18 @@
 // of a sequence with Lq queries and Lk >= Lq keys (the queries are its last
 // tokens). Bound: the matrix cores from some hundred tokens on, 4 head_dim
 // operations per head and visible pair; K and V come from L2. Measured, bf16,
-// GQA 4, 8 KV heads, d128: 1 x 8,192 tokens 482-487 us, 1,130 TFLOP/s (372 with
-// zeros: the chip's power sets the clock), 64 x 512-1,024 477 us, 673 TFLOP/s (6.5
-// key tiles per row block, each with its own start and end), 1 x 517 13.3 us
-// (latency).
+// GQA 4, 8 KV heads, d128: 1 x 8,192 tokens 482-494 us, 1,130 TFLOP/s (372 with
+// zeros: the chip's power sets the clock), 64 x 512-1,024 450 us, 713 TFLOP/s (382
+// with zeros; 6.8 key tiles per row block, each block with its own start and
+// end), 1 x 517 12.3 us (latency).
 //
 //  rows   a workgroup of NW waves takes 32 NW rows of one (sequence, KV head);
 //         row r is query token r / G, head r % G of the group, so that a
 //         group's heads share every K and V tile and a wave's rows span few
 //         tokens (little masked work on the diagonal).
-//         Eight waves per workgroup, or two groups of keys in one, were no faster.
+//         Eight waves per workgroup, two groups of keys in one, or several row
+//         blocks one after the other in one (each's first tile copied during the
+//         last step of the one before) were no faster.
 //  stage  64 tokens of K and V are copied to LDS with global_load_lds (16 B per
 //         lane), double-buffered, one barrier per tile. The 16-byte chunks of
 //         a row are permuted so that the operand reads below meet no bank
