@@ -285,3 +285,74 @@ def test_decode_workspace_refused(rl, gpu):
     for a.workspace, a.workspace_bytes in ((None, 1 << 30), (1 << 20, need - 1)):
         assert rl.lib().rl_hip_attn_decode_kv8(C.byref(a)) == -1
         assert "workspace" in rl.lib().rl_hip_last_error().decode()
+
+
+def test_far_blocks(rl, gpu):
+    """Blocks behind 4 GiB of arena: tokens appended to them and read back by the decode."""
+    rng = np.random.default_rng(32)
+    t, d, kvh, group, n, dtype = 16, 128, 2, 4, 40, "bf16"
+    near = k8.Arena8(6, t, d, fill=False)
+    near_table = rng.permutation(6).astype(np.uint32).reshape(1, kvh, 3)
+    block, ids = near.bytes.shape[1], np.array([3, 1_020_000, 1_020_001, 7, 1_039_998, 1_039_999], np.uint32)
+    assert int(ids[1]) * block > 1 << 32
+    k, v = rows(rng, n, kvh, d, dtype), rows(rng, n, kvh, d, dtype)
+    q = k8.bits(rng.standard_normal((1, kvh * group, d)), dtype)
+    up = rl.DeviceBuffer.from_array
+    arena = rl.DeviceBuffer(1_040_000 * block)
+    table, zero, starts = up(ids[near_table]), up(np.zeros(1, np.uint32)), up(np.array([0, n], np.uint32))
+    kb, vb, qb, ctx = up(k), up(v), up(q), up(np.array([n], np.uint32))
+    out, out32 = rl.DeviceBuffer(q.size * 2), rl.DeviceBuffer(q.size * 4)
+    layout = rl.KvLayoutDesc.paged8(t, d)
+    rl.kv8_append(rl.Kv8AppendArgs(arena_base=arena.ptr, arena_bytes=arena.nbytes, layout=layout, block_table=table.ptr,
+                                   table_stride=3, batch=1, kv_heads=kvh, dtype=rl.DTYPE_BF16, positions=zero.ptr,
+                                   starts=starts.ptr, tokens=n, max_new=n, k_new=kb.ptr, v_new=vb.ptr))
+    args = rl.attn_args(arena, layout, table, 3, 1, kvh * group, kvh, rl.DTYPE_BF16, ctx, 48, qb, out, out32)
+    ws = rl.attn_kv8_workspace(args)
+    rl.attn_decode_kv8(args)
+    rl.sync()
+    fk, fv = k8.floats(k, dtype), k8.floats(v, dtype)
+    for g in range(kvh):
+        near.append(near_table[0, g], 0, np.stack((fk[:, g], fv[:, g])))
+        for j, blk in enumerate(near_table[0, g]):
+            m = min(t, n - j * t)
+            got = arena.download(np.uint8, (block,), int(ids[blk]) * block)
+            assert np.array_equal(got[:near.n].reshape(2, t, d)[:, :m], near.planes(blk)[:, :m])
+            assert np.array_equal(got[near.n:near.n + 8], near.bytes[blk, near.n:near.n + 8])
+    check(near, near_table, [n], q, out.download(np.uint16, q.shape), out32.download(np.float32, q.shape), dtype)
+    for b in (arena, table, zero, starts, kb, vb, qb, ctx, out, out32, ws):
+        b.close()
+
+
+@pytest.mark.parametrize("max_ctx, batch", [(9000, 3), (3300, 80)])
+def test_decode_graphs_share_a_workspace(rl, gpu, max_ctx, batch):
+    """Two captured calls on one workspace, replayed in turn with an eager one between: each as it is alone."""
+    t, d, kvh, group, dtype = 16, 128, 2, 4, "bf16"
+    up, calls, want = rl.DeviceBuffer.from_array, [], []
+    for i in range(3):
+        rng = np.random.default_rng(50 + i)
+        ctx = rng.integers(0, min(max_ctx, 900) + 1, batch).tolist()
+        ctx[0] = max_ctx
+        arena, table, q = decode_case(rng, ctx, kvh, group, t, d, dtype, stride=-(-max_ctx // t), seed=60 + i)
+        want.append(k8.run_decode(rl, arena, table, ctx, q, dtype, max_ctx)[1])
+        dev = [up(arena.bytes), up(table), up(np.asarray(ctx, np.uint32)), up(q), rl.DeviceBuffer(q.size * 2),
+               rl.DeviceBuffer(q.size * 4, zero=True)]
+        calls.append((dev, rl.attn_args(dev[0], rl.KvLayoutDesc.paged8(t, d), dev[1], table.shape[2], batch, kvh * group, kvh,
+                                        rl.DTYPE_BF16, dev[2], max_ctx, dev[3], dev[4], dev[5]), q.shape))
+    ws = rl.attn_kv8_workspace(calls[0][1])
+    for _, args, _ in calls:
+        args.workspace, args.workspace_bytes = ws.ptr, ws.nbytes
+    graphs = [rl.Graph(lambda a=args: rl.attn_decode_kv8(a)) for _, args, _ in calls[:2]]
+    for _ in range(3):
+        graphs[0].launch()
+        rl.attn_decode_kv8(calls[2][1])
+        graphs[1].launch()
+        rl.sync()
+        for (dev, _, shape), ref in zip(calls, want):
+            assert np.array_equal(dev[5].download(np.float32, shape).view(np.uint32), ref.view(np.uint32))
+            rl.check(rl.lib().rl_hip_memset_d(dev[5].ptr, 0, dev[5].nbytes), "memset")
+    for g in graphs:
+        g.close()
+    for dev, _, _ in calls:
+        for b in dev:
+            b.close()
+    ws.close()

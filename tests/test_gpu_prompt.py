@@ -233,6 +233,73 @@ def test_scores_without_weight(rl, gpu):
     assert np.isnan(out[1, 0, 5]) and ok[0].all() and np.delete(ok[1], 5).all()
 
 
+def test_far_tokens(rl, gpu):
+    """The widest strides: tokens of q, k, v and out behind 4 GiB."""
+    rng = np.random.default_rng(33)
+    d, qh, kvh, stride = 128, 4, 1, 1 << 24
+    qs = starts_of([70, 65])
+    n = qs[-1]
+    assert 2 * stride * (n - 1) > 1 << 32
+    q, k, v = inputs(rng, n, n, qh, kvh, d, "bf16")
+    bufs = [rl.DeviceBuffer(2 * stride * (n - 1) + 2 * qh * d) for _ in range(4)]
+    for buf, x in zip(bufs, (q, k, v)):
+        for i in range(n):
+            buf.upload(x[i], 2 * stride * i)
+    sb = rl.DeviceBuffer.from_array(np.array(qs, np.uint32))
+    args = rl.AttnPromptArgs(q=bufs[0].ptr, k=bufs[1].ptr, v=bufs[2].ptr, out=bufs[3].ptr, q_stride=stride, k_stride=stride,
+                             v_stride=stride, out_stride=stride, q_starts=sb.ptr, seqs=2, q_tokens=n, kv_tokens=n, max_q=70,
+                             max_kv=70, q_heads=qh, kv_heads=kvh, head_dim=d, dtype=rl.DTYPE_BF16)
+    ws = rl.attn_prompt_workspace(args)
+    rl.attn_prompt(args)
+    rl.sync()
+    out = np.stack([bufs[3].download(np.uint16, (qh, d), 2 * stride * i) for i in range(n)])
+    compare(out, q, k, v, qs, qs, kvh, "bf16")
+    for b in bufs + [sb, ws]:
+        b.close()
+
+
+def test_graphs_share_a_workspace(rl, gpu):
+    """Two captured calls that share keys among workgroups on one workspace, in turn: each as it is alone."""
+    d, qh, kvh, nq, nk = 128, 8, 2, 3, 2100
+    up, calls, want = rl.DeviceBuffer.from_array, [], []
+    for i in range(2):
+        q, k, v = inputs(np.random.default_rng(70 + i), nq, nk, qh, kvh, d, "bf16")
+        want.append(run(rl, q, k, v, [0, nq], kvh, "bf16", kv_starts=[0, nk]))
+        dev = [up(q), up(k), up(v), up(np.zeros((nq, qh * d), np.uint16)), up(np.array([0, nq], np.uint32)),
+               up(np.array([0, nk], np.uint32))]
+        calls.append((dev, rl.AttnPromptArgs(q=dev[0].ptr, k=dev[1].ptr, v=dev[2].ptr, out=dev[3].ptr, q_starts=dev[4].ptr,
+                                             kv_starts=dev[5].ptr, seqs=1, q_tokens=nq, kv_tokens=nk, max_q=nq, max_kv=nk,
+                                             q_heads=qh, kv_heads=kvh, head_dim=d, dtype=rl.DTYPE_BF16)))
+    ws = rl.attn_prompt_workspace(calls[0][1])
+    assert ws.nbytes > 4096  # (the keys are shared)
+    for _, args in calls:
+        args.workspace, args.workspace_bytes = ws.ptr, ws.nbytes
+    graphs = [rl.Graph(lambda a=args: rl.attn_prompt(a)) for _, args in calls]
+    for _ in range(3):
+        for g in graphs:
+            g.launch()
+        rl.sync()
+        for (dev, _), ref in zip(calls, want):
+            assert np.array_equal(dev[3].download(np.uint16, ref.shape), ref)
+            rl.check(rl.lib().rl_hip_memset_d(dev[3].ptr, 0, dev[3].nbytes), "memset")
+    for g in graphs:
+        g.close()
+    for dev, _ in calls:
+        for b in dev:
+            b.close()
+    ws.close()
+
+
+@pytest.mark.parametrize("short", [0, 1])
+def test_workspace_refusal(rl, gpu, short):
+    a = rl.AttnPromptArgs(q=1 << 20, k=1 << 20, v=1 << 20, out=1 << 20, q_starts=1 << 20, seqs=1, q_tokens=4, kv_tokens=4,
+                          max_q=4, max_kv=4000, q_heads=8, kv_heads=2, head_dim=64, dtype=0)
+    need = rl.attn_prompt_workspace_bytes(a)
+    a.workspace, a.workspace_bytes = (1 << 20, need - 1) if short else (None, need)
+    with pytest.raises(rl.RlrtError, match="workspace"):
+        rl.attn_prompt(a)
+
+
 def test_nothing_to_do(rl, gpu):
     a = rl.AttnPromptArgs(q=1 << 20, k=1 << 20, v=1 << 20, out=1 << 20, q_starts=1 << 20, seqs=1, q_tokens=0, kv_tokens=0,
                           max_q=0, max_kv=0, q_heads=8, kv_heads=2, head_dim=64, dtype=0, workspace=1 << 20,
