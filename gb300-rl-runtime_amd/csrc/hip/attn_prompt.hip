@@ -52,7 +52,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int BT = 64;         // keys per tile
 constexpr int NW = 4;          // waves per workgroup, 32 rows each
 constexpr uint32_t ROWS = NW * 32;
-constexpr uint32_t kShareTiles = 8;  // tiles per workgroup, at least, where several share a row block's keys
+constexpr uint32_t kShareTiles = 6;  // tiles per workgroup, at least, where several share a row block's keys
 constexpr int kPlain = 0, kMasked = 1, kFinal = 2;  // what a step's next scores are: all seen, some hidden, none
 constexpr float kSlack = 8.f;  // log2 of what a weight may exceed its reference by
 
@@ -471,7 +471,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     }
     if constexpr (SPLIT) {
         // (without the steps that have no next scores: with them the compiler
-        // spills the shares' kernel, 24.4 to 34.3 us at 16 queries behind 6,000 keys)
+        // spills the shares' kernel, 10 us more at 16 queries behind 6,000 keys)
         auto turn_if = [&](auto parity, uint32_t s, f32x16 (&cur)[2], f32x16 (&next)[2]) {
             meet(maybe, s, s + 1 < steps);
             if ((first + s) * BT < w_most)
@@ -511,11 +511,14 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     if constexpr (SPLIT)
         part = p.part + (((size_t)at * p.split + blockIdx.x / blocks) * NW + wave) * C::PART;
     if (SPLIT && shares_of(p, nt) > 1) {
+        if (!w_has)
+            return;
 #pragma unroll
         for (int d = 0; d < C::DB; d++)
 #pragma unroll
-            for (int r = 0; r < 16; r++)
-                part[(16 * d + r) * 64 + lane] = o[d][r];
+            for (int a = 0; a < 4; a++)
+                *(rl_f32x4 *)(part + ((4 * d + a) * 64 + lane) * 4) =
+                    rl_f32x4{o[d][4 * a], o[d][4 * a + 1], o[d][4 * a + 2], o[d][4 * a + 3]};
         part[C::DB * 16 * 64 + lane] = m;
         part[(C::DB * 16 + 1) * 64 + lane] = L;
     } else {
@@ -584,7 +587,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
 #pragma unroll
             for (int e = 0; e < E; e++) {  // dim x of row r: see the merge
                 const uint32_t x = lane * E + e;
-                part[(16 * (x / 32) + 4 * (x / 8 % 4) + x % 4) * 64 + 32 * (x / 4 % 2) + r] = acc[e];
+                part[((x / 8) * 64 + 32 * (x / 4 % 2) + r) * 4 + x % 4] = acc[e];
             }
             continue;
         }
@@ -595,23 +598,25 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     }
 }
 
-// Joins the shares of the row blocks that have several: wave `wave` of
-// workgroup `at` the 32 rows that wave `wave` of their workgroups had. Lane l
-// holds, of row l % 32, dim 32 d + 8 (r / 4) + 4 (l / 32) + r % 4 in word 16 d + r.
+// Joins the shares of the row blocks that have several: a workgroup the 32 rows
+// that wave w of theirs had, and 32 of the dims. Lane l holds, of row l % 32, the
+// dims 32 d + 8 j + 4 (l / 32) .. + 3 in its 4 d + j-th four words, which wave j
+// joins, eight shares' loads at a time (one after the other: 23.8 us against 18.7
+// for 16 queries behind 6,000 keys).
 template <int D, int DT>
-__global__ __launch_bounds__(NW * 64) void attn_prompt_merge_kernel(PromptParams p)
+__global__ __launch_bounds__(256) void attn_prompt_merge_kernel(PromptParams p)
 {
     using C = PCfg<D>;
     const int lane = threadIdx.x & 63;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t at = blockIdx.x / C::DB, d = blockIdx.x % C::DB;
+    const uint32_t j = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t d = blockIdx.x % C::DB, w = blockIdx.x / C::DB % NW, at = blockIdx.x / (C::DB * NW);
     uint32_t seq, g, tile;
     block_of(p, at, lane, seq, g, tile);
     const uint32_t qs = rl_sload(p.q_starts + seq), qe = min(rl_sload(p.q_starts + seq + 1), p.q_tokens);
     const uint32_t ks = rl_sload(p.kv_starts + seq), ke = min(rl_sload(p.kv_starts + seq + 1), p.kv_tokens);
     const uint32_t lq = qe > qs ? qe - qs : 0u, lk = ke > ks ? ke - ks : 0u;
     const uint32_t rows = min(lq, p.max_q) * p.group;
-    const uint32_t wg_row = tile * ROWS, row = wg_row + wave * 32 + (lane & 31);
+    const uint32_t wg_row = tile * ROWS, row = wg_row + w * 32 + (lane & 31);
     if (wg_row >= rows)
         return;
     const uint32_t last_tok = quotient(min(wg_row + ROWS, rows) - 1, p.by_group);
@@ -619,38 +624,54 @@ __global__ __launch_bounds__(NW * 64) void attn_prompt_merge_kernel(PromptParams
     const uint32_t n = shares_of(p, (wg_seen + BT - 1) / BT);
     if (n < 2 || row >= rows)
         return;
-    const float *part = p.part + ((size_t)at * p.split * NW + wave) * C::PART + lane;
-    float M = -INFINITY;
-    for (uint32_t i = 0; i < n; i++)
-        M = fmaxf(M, part[(size_t)i * NW * C::PART + C::DB * 16 * 64]);
-    float L = 0.f, o[16];
+    const float *part = p.part + ((size_t)at * p.split * NW + w) * C::PART;
+    const float *tops = part + C::DB * 16 * 64 + lane, *words = part + ((4 * d + j) * 64 + lane) * 4;
+    float M = -INFINITY, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t i0 = 0; i0 < n; i0 += 8) {
+        rl_f32x4 x[8];
+        float m[8], l[8], top = M;
 #pragma unroll
-    for (int r = 0; r < 16; r++)
-        o[r] = 0.f;
-    for (uint32_t i = 0; i < n; i++) {
-        const float *x = part + (size_t)i * NW * C::PART;
-        const float m = x[C::DB * 16 * 64];
-        const float f = m == -INFINITY ? 0.f : exp2f(m - M);
-        L = fmaf(x[(C::DB * 16 + 1) * 64], f, L);
+        for (uint32_t i = 0; i < 8; i++) {
+            const size_t off = (size_t)min(i0 + i, n - 1) * NW * C::PART;
+            x[i] = *(const rl_f32x4 *)(words + off);
+            m[i] = tops[off];
+            l[i] = tops[off + 64];
+        }
 #pragma unroll
-        for (int r = 0; r < 16; r++)
-            o[r] = fmaf(x[(16 * d + r) * 64], f, o[r]);
+        for (uint32_t i = 0; i < 8; i++) {
+            m[i] = i0 + i < n ? m[i] : -INFINITY;
+            top = fmaxf(top, m[i]);
+        }
+        const float keep = M == -INFINITY ? 1.f : exp2f(M - top);  // (before a maximum, sums are 0 or no number)
+        M = top;
+        L *= keep;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            o[e] *= keep;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const float f = m[i] == -INFINITY ? 0.f : exp2f(m[i] - M);
+            if (i0 + i < n) {
+                L = fmaf(l[i], f, L);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    o[e] = fmaf(x[i][e], f, o[e]);
+            }
+        }
     }
     const uint32_t tok = quotient(row, p.by_group), head = g * p.group + row - tok * p.group;
     const bool none = (int32_t)(tok - lq + 1) + (int32_t)lk <= 0;
     const float inv = none ? 0.f : 1.f / L;
-    uint16_t *dst = p.out + (uint64_t)(qs + tok) * p.out_stride + (uint64_t)head * D + 32 * d + 4 * (lane >> 5);
-#pragma unroll
-    for (int a = 0; a < 4; a++)
-        *(rl_u32x2 *)(dst + 8 * a) = rl_u32x2{pack2<DT>(o[4 * a] * inv, o[4 * a + 1] * inv),
-                                             pack2<DT>(o[4 * a + 2] * inv, o[4 * a + 3] * inv)};
+    uint16_t *dst = p.out + (uint64_t)(qs + tok) * p.out_stride + (uint64_t)head * D + 32 * d + 8 * j + 4 * (lane >> 5);
+    *(rl_u32x2 *)dst = rl_u32x2{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
 }
 
-// Few row blocks share their keys, in shares of eight tiles and more, as many as
-// compute units are left: 16 queries behind 6,000 keys 24.4 us against 80.4 of one
-// workgroup per row block, 300 behind 2,000 30.7 against 39.1. With 256 row
-// blocks and more it costs: pieces of four prompts behind 4,000 tokens 74 us,
-// 90 with every row block in two.
+// Few row blocks share their keys, in shares of six tiles and more, as many as
+// compute units are left: 16 queries behind 6,000 keys 17.5 us against 80.4 of one
+// workgroup per row block, 300 behind 2,000 28.9 against 39.1. In shares of eight
+// tiles 18.6 us (16 behind 6,000), of four 18.9. Two shares per compute unit, or
+// row blocks in two from 256 on, cost: 2 x 300 behind 600 23.2 us against 18.1,
+// pieces of four prompts behind 4,000 tokens 90 against 74.
 struct PromptPlan {
     uint32_t tiles, pairs, split;
     size_t workspace;
@@ -681,7 +702,7 @@ int launch(const PromptParams &p)
     hipLaunchKernelGGL((attn_prompt_kernel<D, DT, true>), dim3(grid), dim3(NW * 64), 0, rl_stream(), p);
     if (rl_check_launch("attn_prompt_kernel launch"))
         return -1;
-    hipLaunchKernelGGL((attn_prompt_merge_kernel<D, DT>), dim3(p.pairs * p.tiles * PCfg<D>::DB), dim3(NW * 64), 0,
+    hipLaunchKernelGGL((attn_prompt_merge_kernel<D, DT>), dim3(p.pairs * p.tiles * NW * PCfg<D>::DB), dim3(256), 0,
                        rl_stream(), p);
     return rl_check_launch("attn_prompt_merge_kernel launch");
 }

@@ -221,7 +221,7 @@ def test_scores_without_weight(rl, gpu):
     """A key whose score is minus infinity beside a value that is no number and that the row does not see, with the
     keys shared by several workgroups: the row's other shares give its output."""
     rng = np.random.default_rng(12)
-    nq, nk, finite = 2, 1500, 768  # three shares of eight tiles: the last one's scores are all minus infinity
+    nq, nk, finite = 2, 1500, 768  # the later shares have no score above minus infinity
     q, k, v = inputs(rng, nq, nk, 1, 1, 64, "fp16")
     fq, fk, fv = (k8.floats(x, "fp16") for x in (q, k, v))
     fq[:, :, 0], fk[:finite, 0, 0], fk[finite:, 0, 0], fv[nk - 1, 0, 5] = 1.0, 0.0, -np.inf, np.nan
