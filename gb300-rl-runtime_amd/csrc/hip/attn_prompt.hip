@@ -52,7 +52,8 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int BT = 64;         // keys per tile
 constexpr int NW = 4;          // waves per workgroup, 32 rows each
 constexpr uint32_t ROWS = NW * 32;
-constexpr uint32_t kShareTiles = 6;  // tiles per workgroup, at least, where several share a row block's keys
+// tiles per workgroup, at least, where several share a row block's keys: one and two workgroups per compute unit
+constexpr uint32_t kShareTiles = 6, kLongShareTiles = 48;
 constexpr int kPlain = 0, kMasked = 1, kFinal = 2;  // what a step's next scores are: all seen, some hidden, none
 constexpr float kSlack = 8.f;  // log2 of what a weight may exceed its reference by
 
@@ -669,9 +670,11 @@ __global__ __launch_bounds__(256) void attn_prompt_merge_kernel(PromptParams p)
 // Few row blocks share their keys, in shares of six tiles and more, as many as
 // compute units are left: 16 queries behind 6,000 keys 17.5 us against 80.4 of one
 // workgroup per row block, 300 behind 2,000 28.9 against 39.1. In shares of eight
-// tiles 18.6 us (16 behind 6,000), of four 18.9. Two shares per compute unit, or
-// row blocks in two from 256 on, cost: 2 x 300 behind 600 23.2 us against 18.1,
-// pieces of four prompts behind 4,000 tokens 90 against 74.
+// tiles 18.6 us (16 behind 6,000), of four 18.9. Two shares per compute unit where
+// each still has 48 tiles: 512 behind 32,000 260 us against 280, 2 x 300 behind
+// 16,000 154 against 242 (152 row blocks on 256 compute units); shorter ones
+// cost: 2 x 300 behind 600 23.2 against 18.1. So does it to split more than 256
+// row blocks: 2 x 1,000 behind 4,000 145 against 113.
 struct PromptPlan {
     uint32_t tiles, pairs, split;
     size_t workspace;
@@ -684,8 +687,14 @@ PromptPlan plan_of(const rl_attn_prompt_args_t *a)
     pl.tiles = (uint32_t)(((uint64_t)a->max_q * group + ROWS - 1) / ROWS);
     pl.pairs = a->seqs * a->kv_heads;
     const uint64_t blocks = (uint64_t)pl.tiles * pl.pairs;
-    const uint64_t most = std::max<uint64_t>(1, ((uint64_t)a->max_kv + BT - 1) / BT / kShareTiles);
-    pl.split = blocks == 0 ? 1 : (uint32_t)std::min<uint64_t>(most, std::max<uint64_t>(1, rl_cu_count() / blocks));
+    const uint64_t keys = ((uint64_t)a->max_kv + BT - 1) / BT, cus = rl_cu_count();
+    uint64_t shares = 1;
+    if (blocks > 0 && blocks <= cus) {
+        shares = cus / blocks;
+        if (keys >= kLongShareTiles * (2 * cus / blocks))
+            shares = 2 * cus / blocks;
+    }
+    pl.split = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(shares, keys / kShareTiles));
     const size_t part = (size_t)(a->head_dim / 32 * 16 + 2) * 64 * sizeof(float);
     pl.workspace = 256 + (pl.split > 1 ? (size_t)blocks * pl.split * NW * part : 0);
     return pl;

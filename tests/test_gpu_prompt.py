@@ -102,6 +102,19 @@ def test_many_sequences(rl, gpu):
     compare(out.reshape(q.shape), q, k, v, qs, qs, 3, "bf16")
 
 
+@pytest.mark.parametrize("seqs, longest", [(130, 9300), (200, 6200), (20, 9300)])
+def test_one_long_among_short(rl, gpu, seqs, longest):
+    """More row blocks than half the compute units share the keys of the one long sequence, one or two workgroups each."""
+    rng = np.random.default_rng(seqs)
+    lq, lk = rng.integers(1, 4, seqs), rng.integers(3, 40, seqs)
+    lk[seqs // 3] = longest
+    qs, ks = starts_of(lq.tolist()), starts_of(lk.tolist())
+    q, k, v = inputs(rng, qs[-1], ks[-1], 2, 1, 64, "fp16")
+    out = run(rl, q, k, v, qs, 1, "fp16", kv_starts=ks)
+    compare(out.reshape(q.shape), q, k, v, qs, ks, 1, "fp16")
+    assert np.array_equal(run(rl, q, k, v, qs, 1, "fp16", kv_starts=ks, graph=2), out)
+
+
 @pytest.mark.parametrize("n, kvh", [(1500, 2), (2100, 1)])
 def test_long(rl, gpu, n, kvh):
     rng = np.random.default_rng(n)
