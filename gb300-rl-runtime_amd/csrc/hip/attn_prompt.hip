@@ -87,7 +87,8 @@ struct PromptParams {
     uint32_t pairs;   // sequences x KV heads
     uint32_t tiles;   // row blocks of the longest sequence
     uint32_t by_xcd;  // a pair's row blocks all on one XCD
-    uint32_t ranked;  // the longest sequences first
+    uint32_t ranked;  // the longest sequences first, by ...
+    uint32_t rank_shift;  // ... their keys divided by 2^rank_shift, up to 63
     uint32_t seqs;
     uint32_t split;   // workgroups per row block, at most
     Divisor by_group, by_pairs, by_heads, by_tiles;
@@ -152,50 +153,73 @@ __device__ __forceinline__ float half_sum(float x)
     return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
 
-// The place in the batch of the sequence with the rank-th most keys (ties in
-// batch order), found by every wave for itself: p.seqs <= 64.
-__device__ __forceinline__ uint32_t seq_of_rank(const PromptParams &p, uint32_t rank, int lane)
-{
-    uint32_t n = 0;
-    if ((uint32_t)lane < p.seqs) {
-        const uint32_t a = p.kv_starts[lane], b = min(p.kv_starts[lane + 1], p.kv_tokens);
-        n = b > a ? b - a : 0u;
-    }
-    uint32_t before = 0;
-    for (uint32_t i = 0; i < p.seqs; i++) {
-        const uint32_t x = rl_readlane(n, (int)i);
-        before += x > n || (x == n && i < (uint32_t)lane) ? 1u : 0u;
-    }
-    return (uint32_t)__builtin_ctzll(__builtin_amdgcn_ballot_w64((uint32_t)lane < p.seqs && before == rank));
-}
-
 // The workgroups that share the keys of a row block of nt tiles.
 __device__ __forceinline__ uint32_t shares_of(const PromptParams &p, uint32_t nt)
 {
     return max(1u, min(p.split, nt / kShareTiles));
 }
 
-// Which row block (of 128 rows) of which sequence and KV head workgroup `at` of
-// the grid has: the last ones, which see the most, first, the longest
-// sequences first, and all of a pair's on one XCD (workgroup b runs on XCD b %
-// 8), behind whose L2 they share K and V.
-__device__ __forceinline__ void block_of(const PromptParams &p, uint32_t at, int lane, uint32_t &seq, uint32_t &g,
-                                         uint32_t &tile)
+// The lane whose key, 0 to 63, is the rank-th largest of the first n lanes (ties
+// in lane order): the largest value that more than `rank` keys reach, bit by bit.
+__device__ __forceinline__ uint32_t lane_of_rank(uint32_t key, uint32_t n, uint32_t rank)
 {
+    const uint64_t lanes = ~0ull >> (64 - n);
+    uint32_t least = 0;
+#pragma unroll
+    for (uint32_t bit = 32; bit > 0; bit /= 2)
+        if ((uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key >= (least | bit)) & lanes) > rank)
+            least |= bit;
+    const uint64_t same = __builtin_amdgcn_ballot_w64(key == least) & lanes;
+    const uint32_t more = (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key > least) & lanes);
+    const uint32_t before = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
+    return (uint32_t)__builtin_ctzll(__builtin_amdgcn_ballot_w64(before == rank - more) & same);
+}
+
+// A workgroup's row block (of 128 rows): the tile-th of a sequence and KV head g,
+// whose queries start at qs, lq of them, and the keys at ks.
+struct Place {
+    uint32_t g, tile, qs, lq, ks, lk;
+};
+
+// Which one workgroup `at` of the grid has: the last ones, which see the most,
+// first, the longest sequences first, and all of a pair's on one XCD (workgroup
+// b runs on XCD b % 8), behind whose L2 they share K and V.
+__device__ __forceinline__ Place place_of(const PromptParams &p, uint32_t at, int lane)
+{
+    Place x;
     uint32_t pair;
     if (p.by_xcd) {
         const uint32_t local = at / 8, n = quotient(local, p.by_tiles);
         pair = at % 8 + 8 * n;
-        tile = p.tiles - 1 - (local - n * p.tiles);
+        x.tile = p.tiles - 1 - (local - n * p.tiles);
     } else {
         const uint32_t n = quotient(at, p.by_pairs);
         pair = at - n * p.pairs;
-        tile = p.tiles - 1 - n;
+        x.tile = p.tiles - 1 - n;
     }
-    seq = quotient(pair, p.by_heads);
-    g = pair - seq * p.kv_heads;
-    if (p.ranked)
-        seq = seq_of_rank(p, seq, lane);
+    const uint32_t seq = quotient(pair, p.by_heads);
+    x.g = pair - seq * p.kv_heads;
+    uint32_t qe, ke;
+    if (p.ranked) {
+        const uint32_t i = min((uint32_t)lane, p.seqs - 1);
+        const uint32_t q0 = p.q_starts[i], q1 = p.q_starts[i + 1], k0 = p.kv_starts[i], k1 = p.kv_starts[i + 1];
+        const uint32_t n = min(k1, p.kv_tokens);
+        const int l = (int)lane_of_rank(min((n > k0 ? n - k0 : 0u) >> p.rank_shift, 63u), p.seqs, seq);
+        x.qs = rl_readlane(q0, l);
+        qe = rl_readlane(q1, l);
+        x.ks = rl_readlane(k0, l);
+        ke = rl_readlane(k1, l);
+    } else {
+        x.qs = rl_sload(p.q_starts + seq);
+        qe = rl_sload(p.q_starts + seq + 1);
+        x.ks = rl_sload(p.kv_starts + seq);
+        ke = rl_sload(p.kv_starts + seq + 1);
+    }
+    qe = min(qe, p.q_tokens);
+    ke = min(ke, p.kv_tokens);
+    x.lq = qe > x.qs ? qe - x.qs : 0u;
+    x.lk = ke > x.ks ? ke - x.ks : 0u;
+    return x;
 }
 
 // One row block; SPLIT: or a share of its keys, its sums to the workspace.
@@ -210,11 +234,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t hf = (uint32_t)lane >> 5;
     const uint32_t blocks = p.pairs * p.tiles, at = SPLIT ? blockIdx.x % blocks : blockIdx.x;
-    uint32_t seq, g, tile;
-    block_of(p, at, lane, seq, g, tile);
-    const uint32_t qs = rl_sload(p.q_starts + seq), qe = min(rl_sload(p.q_starts + seq + 1), p.q_tokens);
-    const uint32_t ks = rl_sload(p.kv_starts + seq), ke = min(rl_sload(p.kv_starts + seq + 1), p.kv_tokens);
-    const uint32_t lq = qe > qs ? qe - qs : 0u, lk = ke > ks ? ke - ks : 0u;
+    const Place x = place_of(p, at, lane);
+    const uint32_t g = x.g, tile = x.tile, qs = x.qs, lq = x.lq, ks = x.ks, lk = x.lk;
     const uint32_t rows = min(lq, p.max_q) * p.group, wg_row = tile * ROWS;
     if (wg_row >= rows)
         return;
@@ -611,11 +632,8 @@ __global__ __launch_bounds__(256) void attn_prompt_merge_kernel(PromptParams p)
     const int lane = threadIdx.x & 63;
     const uint32_t j = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t d = blockIdx.x % C::DB, w = blockIdx.x / C::DB % NW, at = blockIdx.x / (C::DB * NW);
-    uint32_t seq, g, tile;
-    block_of(p, at, lane, seq, g, tile);
-    const uint32_t qs = rl_sload(p.q_starts + seq), qe = min(rl_sload(p.q_starts + seq + 1), p.q_tokens);
-    const uint32_t ks = rl_sload(p.kv_starts + seq), ke = min(rl_sload(p.kv_starts + seq + 1), p.kv_tokens);
-    const uint32_t lq = qe > qs ? qe - qs : 0u, lk = ke > ks ? ke - ks : 0u;
+    const Place place = place_of(p, at, lane);
+    const uint32_t g = place.g, tile = place.tile, qs = place.qs, lq = place.lq, lk = place.lk;
     const uint32_t rows = min(lq, p.max_q) * p.group;
     const uint32_t wg_row = tile * ROWS, row = wg_row + w * 32 + (lane & 31);
     if (wg_row >= rows)
@@ -829,9 +847,12 @@ extern "C" int rl_hip_attn_prompt(const rl_attn_prompt_args_t *a)
     p.by_tiles = divisor_of(p.tiles);
     p.part = (float *)a->workspace;
     p.by_xcd = p.pairs % 8 == 0;
-    // (longest sequences first: 9 of 3-2,047 tokens, d64, 31.5 us, 36 in batch order; each
-    // workgroup ranks for itself, so not for long lists)
+    // (each workgroup finds its place for itself: 9 of 3-2,047 tokens, d64, 31 us against 37 in
+    // batch order; with many row blocks it costs: 64 of 512-1,024 tokens 446 us against 437)
     p.ranked = p.seqs > 1 && p.seqs <= 64 && (uint64_t)p.pairs * p.tiles <= 4096;
+    p.rank_shift = 0;
+    while (a->max_kv >> p.rank_shift > 63)
+        p.rank_shift++;
     if (a->head_dim == 128)
         return a->dtype == RL_DTYPE_BF16 ? launch<128, 0>(p) : launch<128, 1>(p);
     return a->dtype == RL_DTYPE_BF16 ? launch<64, 0>(p) : launch<64, 1>(p);
