@@ -102,6 +102,18 @@ def test_many_sequences(rl, gpu):
     compare(out.reshape(q.shape), q, k, v, qs, qs, 3, "bf16")
 
 
+@pytest.mark.parametrize("seqs", [2, 63, 64])
+def test_sequences_in_order(rl, gpu, seqs):
+    """As many sequences as are put in order, by lengths that are equal, nearly equal, none and far apart."""
+    rng = np.random.default_rng(seqs)
+    lens = rng.choice([0, 1, 2, 30, 31, 64, 130], seqs)
+    lens[seqs - 1] = 700
+    qs = starts_of(lens.tolist())
+    q, k, v = inputs(rng, qs[-1], qs[-1], 4, 2, 64, "bf16")
+    out = run(rl, q, k, v, qs, 2, "bf16")
+    compare(out.reshape(q.shape), q, k, v, qs, qs, 2, "bf16")
+
+
 @pytest.mark.parametrize("seqs, longest", [(130, 9300), (200, 6200), (20, 9300)])
 def test_one_long_among_short(rl, gpu, seqs, longest):
     """More row blocks than half the compute units share the keys of the one long sequence, one or two workgroups each."""
