@@ -45,6 +45,7 @@ namespace {
 
 constexpr int kUnit = 32;           // tokens per unit
 constexpr uint32_t kRowCost = 8;    // units that turning to a row is worth
+constexpr uint64_t kKeptBytes = 256u << 20;  // what the last cache before HBM holds
 
 struct Kv8Params {
     const uint8_t *arena;
@@ -216,12 +217,23 @@ __device__ __forceinline__ Window8<TPB> window8(const Kv8Params &p, uint32_t row
     return win;
 }
 
+// A load of the cache; ONCE: of bytes that nobody reads again soon, which the
+// caches need not keep.
+template <bool ONCE, class T>
+__device__ __forceinline__ T cache_load(const uint8_t *p)
+{
+    if constexpr (ONCE)
+        return __builtin_nontemporal_load((const T *)p);
+    else
+        return *(const T *)p;
+}
+
 // Units u0 .. u1 - 1 of row (rollout b, KV head g) by the W waves of a
 // workgroup: the row's output when part is NULL, else a partial. lds: [W][G * D
 // + 2 G] floats, free again when the last wave returns from a later barrier.
 // win: the wave's first table entries (window8), loaded by the caller as early
 // as it can.
-template <int D, int DT, int TPB, int W>
+template <int D, int DT, int TPB, int W, bool ONCE>
 __device__ __forceinline__ void attend8(const Kv8Params &p, uint32_t b, uint32_t g, uint32_t cin, uint32_t u0,
                                         uint32_t u1, Window8<TPB> win, float *part, float *lds)
 {
@@ -295,7 +307,7 @@ __device__ __forceinline__ void attend8(const Kv8Params &p, uint32_t b, uint32_t
                 const uint8_t *at = BPU == 2 ? base[i % BPU] : base[0] + i * 16 * D;
 #pragma unroll
                 for (int q = 0; q < D / 64; q++)
-                    u.k[i][q] = *(const rl_u32x4 *)(at + koff + 64 * q);
+                    u.k[i][q] = cache_load<ONCE, rl_u32x4>(at + koff + 64 * q);
                 // (a vector load: these return in order, so the unit in flight is not waited for)
                 u.scale[i] = *(const rl_f32x2 *)(base[i % BPU] + 2 * TPB * D + zero);
             }
@@ -305,11 +317,11 @@ __device__ __forceinline__ void attend8(const Kv8Params &p, uint32_t b, uint32_t
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     if constexpr (D == 128) {
-                        const rl_u32x2 x = *(const rl_u32x2 *)(at + voff + r * D);
+                        const rl_u32x2 x = cache_load<ONCE, rl_u32x2>(at + voff + r * D);
                         u.v[4 * i + r][0] = x[0];
                         u.v[4 * i + r][D / 64 - 1] = x[1];
                     } else {
-                        u.v[4 * i + r][0] = *(const uint32_t *)(at + voff + r * D);
+                        u.v[4 * i + r][0] = cache_load<ONCE, uint32_t>(at + voff + r * D);
                     }
                 }
             }
@@ -418,15 +430,31 @@ __global__ __launch_bounds__(W * 64) void attn_kv8_rows_kernel(Kv8Params p)
     const uint32_t u0 = (uint32_t)((uint64_t)s * nu / n), u1 = (uint32_t)((uint64_t)(s + 1) * nu / n);
     if (p.split > 1)
         win = window8<TPB, W>(p, row, u0, 0);
-    attend8<D, DT, TPB, W>(p, b, g, cin, u0, u1, win,
-                           n > 1 ? p.part + (size_t)wg * (p.group * D + 2 * p.group) : nullptr, lds);
+    attend8<D, DT, TPB, W, false>(p, b, g, cin, u0, u1, win,
+                                  n > 1 ? p.part + (size_t)wg * (p.group * D + 2 * p.group) : nullptr, lds);
+}
+
+// Whether a rollout beside b begins with the same block, as those that share a
+// prompt do.
+__device__ __forceinline__ bool shares_blocks(const Kv8Params &p, uint32_t b, uint32_t g)
+{
+    const uint32_t *first = p.table + (size_t)g * p.table_stride;
+    const size_t step = (size_t)p.kv_heads * p.table_stride;
+    const uint32_t here = rl_sload(first + b * step);
+    return (b > 0 && rl_sload(first + (b - 1) * step) == here) ||
+           (b + 1 < p.batch && rl_sload(first + (b + 1) * step) == here);
 }
 
 // ---- many rows: the units of all rows in even shares -----------------------------
 // The units of all rows, rows in (b, g) order, form one sequence; the
 // workgroups, two per compute unit, take equal runs of it, whatever the
 // contexts are. A run that covers a row writes its output; a row that several
-// share is merged from their partials. A workgroup has at most two of those, of
+// share is merged from their partials. Where all rows are more than the last
+// cache keeps for a next call, the rows of rollouts that share no prompt with
+// their neighbours are read past the caches (8 x 32,768 tokens, 539 MB, 94.5 us
+// against 104; 64 x 512-4,096, 304 MB, 62 against 67. What is kept pays below: 64
+// x 1,536 again and again 35.6 against 37.4; and with shared prompts: 64 x 4,096,
+// three quarters shared by eight, 67 against 82). A workgroup has at most two of those, of
 // the rows its run starts and ends in: number 2 w when the row's part starts
 // the run, else 2 w + 1.
 template <int D, int DT, int TPB, int W>
@@ -470,13 +498,18 @@ __global__ __launch_bounds__(W * 64) void attn_kv8_even_kernel(Kv8Params p)
         return;
     uint32_t cin = rl_sload(p.ctx + b), nu = units_of(p, cin);
     uint32_t g = (first - before) / cost_of(nu), x = (first - before) % cost_of(nu);  // x: of this row's cost
+    const bool once = (uint64_t)total * (2 * kUnit * D) > kKeptBytes;
     uint32_t parts = 0;
     for (uint32_t at = first; at < last;) {
         const uint32_t m = min(cost_of(nu) - x, last - at);
         const uint32_t u0 = max(x, kRowCost) - kRowCost, u1 = max(x + m, kRowCost) - kRowCost;
         if (u1 > u0) {
-            attend8<D, DT, TPB, W>(p, b, g, cin, u0, u1, window8<TPB, W>(p, b * p.kv_heads + g, u0, 0),
-                                   u1 - u0 < nu ? p.part + (size_t)(2 * wg + min(parts, 1u)) * PART : nullptr, lds);
+            const Window8<TPB> win = window8<TPB, W>(p, b * p.kv_heads + g, u0, 0);
+            float *part = u1 - u0 < nu ? p.part + (size_t)(2 * wg + min(parts, 1u)) * PART : nullptr;
+            if (once && !shares_blocks(p, b, g))
+                attend8<D, DT, TPB, W, true>(p, b, g, cin, u0, u1, win, part, lds);
+            else
+                attend8<D, DT, TPB, W, false>(p, b, g, cin, u0, u1, win, part, lds);
             parts++;
             __syncthreads();
         }

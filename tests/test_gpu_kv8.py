@@ -356,3 +356,20 @@ def test_decode_graphs_share_a_workspace(rl, gpu, max_ctx, batch):
         for b in dev:
             b.close()
     ws.close()
+
+
+@pytest.mark.parametrize("t, d, kvh, n, dtype", [(16, 128, 8, 7800, "bf16"), (32, 64, 16, 7900, "fp16")])
+def test_decode_more_than_the_caches_keep(rl, gpu, t, d, kvh, n, dtype):
+    """More than 256 MiB of cache, a part of it prompts that neighbours share: alone, first, last and between."""
+    rng = np.random.default_rng(d)
+    ctx = (n + rng.integers(0, 1000, 18)).tolist()
+    ctx[5] = 0
+    arena, table, q = decode_case(rng, ctx, kvh, 2, t, d, dtype)
+    assert 2 * d * kvh * sum(ctx) > 256 << 20
+    shared = n // t // 2
+    for b in (1, 9, 10, 17):  # with the one before
+        table[b, :, :shared] = table[b - 1, :, :shared]
+    out16, out32 = k8.run_decode(rl, arena, table, ctx, q, dtype, max(ctx))
+    rows = [0, 1, 4, 6, 9, 10, 11, 16, 17]
+    check(arena, table[rows], np.array(ctx)[rows], q[rows], out16[rows], out32[rows], dtype)
+    assert not out32[5].any()
