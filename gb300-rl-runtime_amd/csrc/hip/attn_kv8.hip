@@ -6,8 +6,8 @@
 // with sK(t), sV(t) the scales of token t's block. Bound: the bytes of the
 // cache, 2 head_dim per token and KV head; for few rows the chain context,
 // table, block, MFMA, merge. Measured, bf16, GQA 4, 8 KV heads, d128: 8 x 32,768
-// tokens (539 MB) 103 us, 64 x 512-4,096 (304 MB) 66.5 us; equal contexts fit 5.8
-// us plus 5.6 TB/s. 1 x 517 tokens 8.0 us, 24 x 64-2,048 of d64 11.0 us.
+// tokens (539 MB) 94.5 us, 64 x 512-4,096 (304 MB) 62.2 us; 5.8 us of it are there
+// for the shortest contexts too. 1 x 517 tokens 8.0 us, 24 x 64-2,048 of d64 11.0 us.
 //
 //  work   a row (rollout, KV head) is ceil(ctx / 32) units of 32 tokens. Few
 //         rows have workgroups of their own, many rows are cut in even shares

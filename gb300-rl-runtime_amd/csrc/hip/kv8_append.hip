@@ -14,9 +14,11 @@
 // One wave per (row, block, KV head): a lane holds eight elements of every
 // 512 / head_dim-th token of both planes, so that a block is read once, its
 // largest magnitudes are reduced across the wave in registers, and the bytes
-// leave in 8-byte stores. Bound: the bytes, 2 in and 1 out per element (64
-// prompts of 512-1,024 tokens, 302 MB in 65 us: 4.65 TB/s, 91% of a plain
-// copy); for one token per row the chain position, table entry, scale, store
+// leave in 8-byte stores. The rows are read past the caches, for this is their
+// last use (60.9 us against 65.2 below); the blocks are not written past them
+// (58.2), for the next decode step reads them. Bound: the bytes, 2 in and 1 out
+// per element (64 prompts of 512-1,024 tokens, 302 MB in 60.9 us: 4.95 TB/s, 97%
+// of a plain copy); for one token per row the chain position, table entry, scale, store
 // (64 rows x 8 heads: 4.2 us).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -106,8 +108,8 @@ __global__ __launch_bounds__(kWaves * 64) void kv8_append_kernel(Append8Params p
         kw[i] = vw[i] = rl_u32x4{0, 0, 0, 0};
         if (slot >= lo && slot < hi) {
             const uint64_t t = tok0 + (slot - lo);
-            kw[i] = *(const rl_u32x4 *)(p.k_new + t * p.k_stride + g * D + c * 8);
-            vw[i] = *(const rl_u32x4 *)(p.v_new + t * p.v_stride + g * D + c * 8);
+            kw[i] = __builtin_nontemporal_load((const rl_u32x4 *)(p.k_new + t * p.k_stride + g * D + c * 8));
+            vw[i] = __builtin_nontemporal_load((const rl_u32x4 *)(p.v_new + t * p.v_stride + g * D + c * 8));
         }
     }
     // the block that holds the earlier tokens: this one, or the shared one that is copied
