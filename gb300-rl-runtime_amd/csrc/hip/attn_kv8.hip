@@ -449,14 +449,17 @@ __device__ __forceinline__ bool shares_blocks(const Kv8Params &p, uint32_t b, ui
 // The units of all rows, rows in (b, g) order, form one sequence; the
 // workgroups, two per compute unit, take equal runs of it, whatever the
 // contexts are. A run that covers a row writes its output; a row that several
-// share is merged from their partials. Where all rows are more than the last
-// cache keeps for a next call, the rows of rollouts that share no prompt with
-// their neighbours are read past the caches (8 x 32,768 tokens, 539 MB, 94.5 us
-// against 104; 64 x 512-4,096, 304 MB, 62 against 67. What is kept pays below: 64
-// x 1,536 again and again 35.6 against 37.4; and with shared prompts: 64 x 4,096,
-// three quarters shared by eight, 67 against 82). A workgroup has at most two of those, of
+// share is merged from their partials. A workgroup has at most two of those, of
 // the rows its run starts and ends in: number 2 w when the row's part starts
 // the run, else 2 w + 1.
+// Where all rows are more than the last cache keeps for a next call, the rows of
+// rollouts that share no prompt with their neighbours are read past the caches:
+// 8 x 32,768 tokens (539 MB) 94.5 us against 104, and 109 against 116 behind a
+// product with 1 GiB of weights, as in a model's step; 64 x 512-4,096 (304 MB) 62
+// against 67. What is kept pays below (64 x 1,536 again and again 35.6 against
+// 37.4), with shared prompts (64 x 4,096, three quarters shared by eight, 67
+// against 82), and right behind 1 GiB of writes, which the last cache still has to
+// put away (107 against 140): that last one the kernel cannot see.
 template <int D, int DT, int TPB, int W>
 __global__ __launch_bounds__(W * 64) void attn_kv8_even_kernel(Kv8Params p)
 {

@@ -15,11 +15,12 @@
 // 512 / head_dim-th token of both planes, so that a block is read once, its
 // largest magnitudes are reduced across the wave in registers, and the bytes
 // leave in 8-byte stores. The rows are read past the caches, for this is their
-// last use (60.9 us against 65.2 below); the blocks are not written past them
-// (58.2), for the next decode step reads them. Bound: the bytes, 2 in and 1 out
-// per element (64 prompts of 512-1,024 tokens, 302 MB in 60.9 us: 4.95 TB/s, 97%
-// of a plain copy); for one token per row the chain position, table entry, scale, store
-// (64 rows x 8 heads: 4.2 us).
+// last use (60.9 us against 65.2 below, 57 against 62 for rows that were just
+// written); the blocks are not written past them (58.2), for the next decode
+// step reads them. Bound: the bytes, 2 in and 1 out per element (64 prompts of
+// 512-1,024 tokens, 302 MB in 60.9 us: 4.95 TB/s, 97% of a plain copy); for one
+// token per row the chain position, table entry, scale, store (64 rows x 8
+// heads: 4.2 us).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
