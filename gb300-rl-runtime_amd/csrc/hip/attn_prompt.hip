@@ -522,32 +522,32 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     }
     rl_wait_vmcnt<0>();
     const float L = half_sum(l + l2);
-    // ---- the rows' outputs -------------------------------------------------------
     float odd = 0.f;
 #pragma unroll
     for (int d = 0; d < C::DB; d++)
 #pragma unroll
         for (int r = 0; r < 16; r++)
             odd = fmaf(o[d][r], 0.f, odd);
-    float *part = nullptr;
-    if constexpr (SPLIT)
-        part = p.part + (((size_t)at * p.split + blockIdx.x / blocks) * NW + wave) * C::PART;
-    if (SPLIT && shares_of(p, nt) > 1) {
-        if (!w_has)
-            return;
+    // ---- the rows' outputs -------------------------------------------------------
+    auto put = [&] {
+        if constexpr (SPLIT) {
+            if (shares_of(p, nt) > 1) {
+                float *part = p.part + (((size_t)at * p.split + blockIdx.x / blocks) * NW + wave) * C::PART;
 #pragma unroll
-        for (int d = 0; d < C::DB; d++)
+                for (int d = 0; d < C::DB; d++)
 #pragma unroll
-            for (int a = 0; a < 4; a++)
-                *(rl_f32x4 *)(part + ((4 * d + a) * 64 + lane) * 4) =
-                    rl_f32x4{o[d][4 * a], o[d][4 * a + 1], o[d][4 * a + 2], o[d][4 * a + 3]};
-        part[C::DB * 16 * 64 + lane] = m;
-        part[(C::DB * 16 + 1) * 64 + lane] = L;
-    } else {
+                    for (int a = 0; a < 4; a++)
+                        *(rl_f32x4 *)(part + ((4 * d + a) * 64 + lane) * 4) =
+                            rl_f32x4{o[d][4 * a], o[d][4 * a + 1], o[d][4 * a + 2], o[d][4 * a + 3]};
+                part[C::DB * 16 * 64 + lane] = m;
+                part[(C::DB * 16 + 1) * 64 + lane] = L;
+                return;
+            }
+        }
         const float inv = my_seen == 0 ? 0.f : 1.f / L;
         uint16_t *out = p.out + (uint64_t)(qs + tok0) * p.out_stride + (uint64_t)g * p.group * D;
         const uint32_t r = (uint32_t)lane & 31u, dt = quotient(h0 + r, p.by_group);
-        const uint32_t at = dt * (uint32_t)p.out_stride + (h0 + r - dt * p.group) * D + 8 * hf;
+        const uint32_t to = dt * (uint32_t)p.out_stride + (h0 + r - dt * p.group) * D + 8 * hf;
         const bool has = w_row + r < rows;
 #pragma unroll
         for (int d = 0; d < C::DB; d++)
@@ -564,59 +564,116 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
                     w[2 + e] = h[1];
                 }
                 if (has)
-                    *(rl_u32x4 *)(out + at + 32 * d + 8 * a) = w;
+                    *(rl_u32x4 *)(out + to + 32 * d + 8 * a) = w;
             }
-    }
-    // A value of V that is no number spoils its whole 64-key tile in the matrix
-    // product, also for the rows that do not see it (0 times NaN). Rows with
-    // such an output are computed again, key by key, over what they see. (A
-    // row whose sum is no number is right as it is: NaN.)
-    uint64_t again = __builtin_amdgcn_ballot_w64(odd != 0.f && L == L && w_row + (lane & 31) < rows);
-    again = (again | again >> 32) & 0xFFFFFFFFu;
-    if (again)
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (other lanes' stores to the same places came first)
-    while (again) {
-        const int r = __builtin_ctzll(again);
-        again &= again - 1;
-        const uint32_t dt = quotient(h0 + r, p.by_group), tok = tok0 + dt, head = g * p.group + h0 + r - dt * p.group;
-        const uint32_t n = rl_readlane(my_seen, r);
-        const float mr = __uint_as_float(rl_readlane(__float_as_uint(m), r)), neg = mr == -INFINITY ? 0.f : -mr;
-        const float lr = __uint_as_float(rl_readlane(__float_as_uint(L), r));
+    };
+    if (w_has)
+        put();
+    // ---- values that are no numbers -------------------------------------------------
+    // (a row whose sum is no number is right as it is: NaN)
+    if (__builtin_amdgcn_ballot_w64(odd != 0.f && L == L && w_row + (lane & 31) < rows) != 0) {
+        // An infinity or NaN in V spoils its whole tile in the matrix product, also
+        // for the rows that do not see it (0 times NaN). Below `whole` every row sees
+        // every key, so what came of those tiles is right; the keys from there to
+        // `held` are at most two tiles' and are looked through. Where they hold only
+        // numbers the outputs stand. (In fp16 a weight below 2^-25 is rounded to 0, and
+        // 0 times a seen infinity is NaN instead: such outputs are computed again too.)
+        // 1 x 8,192 tokens, 480-500 us (fp16 520) without any: a NaN in the first token
+        // 501 (fp16 4,700), in the last 2,070 (fp16 2,600), an infinity in a dim of every
+        // token 3,800 (fp16 4,700); 16 queries behind 6,000 keys 18 without, 28 (fp16 90),
+        // 70 (fp16 116), 69 (fp16 115).
+        const uint32_t whole = max(w_least, first * BT), held = min((w_most + BT - 1) / BT * BT, lk);
         constexpr int E = D / 64;  // dims per lane
-        const uint16_t *q = p.q + (uint64_t)(qs + tok) * p.q_stride + (uint64_t)head * D + lane * E;
-        float qv[E], acc[E];
+        float spoilt = 0.f;
+        for (uint32_t j = whole; j < held; j += 8)
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            qv[e] = from16<DT>(q[e]);
-            acc[e] = 0.f;
-        }
-        for (uint32_t j = first * BT; j < n; j++) {
-            const uint16_t *kr = kbase + (uint64_t)j * p.k_stride + lane * E;
-            const uint16_t *vr = vbase + (uint64_t)j * p.v_stride + lane * E;
-            float s = 0.f;
+            for (uint32_t i = 0; i < 8; i++) {
+                const uint16_t *x = vbase + (uint64_t)min(j + i, held - 1) * p.v_stride + lane * E;
 #pragma unroll
-            for (int e = 0; e < E; e++)
-                s = fmaf(qv[e], from16<DT>(kr[e]), s);
-#pragma unroll
-            for (int x = 1; x < 64; x *= 2)
-                s += __shfl_xor(s, x);
-            const float w = __builtin_amdgcn_exp2f(fmaf(s, p.scale_log2, neg));
-#pragma unroll
-            for (int e = 0; e < E; e++)
-                acc[e] = fmaf(w, from16<DT>(vr[e]), acc[e]);
-        }
-        if (SPLIT && shares_of(p, nt) > 1) {
-#pragma unroll
-            for (int e = 0; e < E; e++) {  // dim x of row r: see the merge
-                const uint32_t x = lane * E + e;
-                part[((x / 8) * 64 + 32 * (x / 4 % 2) + r) * 4 + x % 4] = acc[e];
+                for (int e = 0; e < E; e++)
+                    spoilt = fmaf(from16<DT>(x[e]), 0.f, spoilt);
             }
-            continue;
-        }
-        uint16_t *dst = p.out + (uint64_t)(qs + tok) * p.out_stride + (uint64_t)head * D + lane * E;
+        if constexpr (DT != 0) {
 #pragma unroll
-        for (int e = 0; e < E; e++)
-            dst[e] = n ? to16<DT>(acc[e] / lr) : (uint16_t)0;
+            for (int d = 0; d < C::DB; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    spoilt = L == L && o[d][r] != o[d][r] ? o[d][r] : spoilt;
+        }
+        if (__builtin_amdgcn_ballot_w64(spoilt != 0.f) != 0) {
+            // The wave's rows again, from memory: 32 keys at a time by the matrix
+            // cores while all rows see them, then key by key for those that do.
+            const float neg = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+            for (int d = 0; d < C::DB; d++)
+                o[d] = f32x16{};
+            uint32_t j = first * BT;
+            for (; j + 32 <= whole; j += 32) {
+                const uint16_t *kp = kbase + (uint64_t)(j + kr) * p.k_stride + 8 * hf;
+                f32x16 x{};
+#pragma unroll
+                for (int s = 0; s < C::KS; s++)
+                    x = mfma32<DT>(*(const s16x8 *)(kp + 16 * s), qf[s], x);
+                float w[16];
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    w[r] = __builtin_amdgcn_exp2f(fmaf(x[r], p.scale_log2, neg));
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    // Weights and values as bf16, whose exponents reach every weight: the
+                    // weights' high and low parts (low ones times numbers only), fp16 values'
+                    // too, so that nothing of them is lost.
+                    s16x8 wh, wl;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        wh[e] = (short)to16<0>(w[8 * u + e]);
+                        wl[e] = (short)to16<0>(w[8 * u + e] - from16<0>((uint16_t)wh[e]));
+                    }
+                    const uint16_t *vp = vbase + (uint64_t)(j + 16 * u + 4 * hf) * p.v_stride + (lane & 31);
+#pragma unroll
+                    for (int d = 0; d < C::DB; d++) {
+                        s16x8 vh, vl, vn;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const float v = from16<DT>(vp[(uint64_t)(e % 4 + 8 * (e / 4)) * p.v_stride + 32 * d]);
+                            vh[e] = (short)to16<0>(v);
+                            const bool number = v * 0.f == 0.f;
+                            vn[e] = number ? vh[e] : (short)0;
+                            vl[e] = number ? (short)to16<0>(v - from16<0>((uint16_t)vh[e])) : (short)0;
+                        }
+                        o[d] = mfma32<0>(vh, wh, o[d]);
+                        o[d] = mfma32<0>(vn, wl, o[d]);
+                        if constexpr (DT != 0)
+                            o[d] = mfma32<0>(vl, wh, o[d]);
+                    }
+                }
+            }
+            for (; j < w_most; j++) {
+                const uint16_t *kp = kbase + (uint64_t)j * p.k_stride + 8 * hf;
+                const uint16_t *vp = vbase + (uint64_t)j * p.v_stride + 4 * hf;
+                float x = 0.f;
+#pragma unroll
+                for (int s = 0; s < C::KS; s++) {
+                    const s16x8 k = *(const s16x8 *)(kp + 16 * s);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        x = fmaf(from16<DT>((uint16_t)k[e]), from16<DT>((uint16_t)qf[s][e]), x);
+                }
+                const float w = __builtin_amdgcn_exp2f(fmaf(half_sum(x), p.scale_log2, neg));
+                if (j < my_seen) {
+#pragma unroll
+                    for (int d = 0; d < C::DB; d++)
+#pragma unroll
+                        for (int a = 0; a < 4; a++) {
+                            const s16x4 v = *(const s16x4 *)(vp + 32 * d + 8 * a);
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                o[d][4 * a + e] = fmaf(w, from16<DT>((uint16_t)v[e]), o[d][4 * a + e]);
+                        }
+                }
+            }
+            put();  // (each lane to the places it wrote before)
+        }
     }
 }
 

@@ -136,7 +136,9 @@ int rl_hip_attn_decode(const rl_attn_decode_args_t *args);
  * (q_heads / kv_heads). out = softmax(scale q K^T) V with fp32 sums, the
  * weights rounded to the inputs' type, stored in it. A query that sees no key
  * (Lk < Lq) yields zeros. What a query does not see has no part in its output,
- * NaN and infinities included. Rows of out that belong to no sequence are left
+ * NaN and infinities included; where they stand among a row's last keys, or
+ * fp16 yields NaN, the row is computed a second time (a call whose rows all are
+ * takes up to ten times as long). Rows of out that belong to no sequence are left
  * as they were; rows of q, k and v past q_tokens and kv_tokens are never read.
  * out may not overlap the inputs. */
 typedef struct {

@@ -206,6 +206,81 @@ def test_shares_and_what_is_not_seen(rl, gpu):
     assert same[seen].all()
 
 
+@pytest.mark.parametrize("dtype, d", [("bf16", 128), ("fp16", 128), ("fp16", 64), ("bf16", 64)])
+def test_values_that_are_no_numbers_early(rl, gpu, dtype, d):
+    """A NaN in a value that every row sees, one that only the later ones see, infinities beside them and in every value of
+    a dim: each in its own dims, all the others as without them."""
+    rng = np.random.default_rng(17)
+    n, qh, qs = 1300, 4, [0, 1300]
+    q, k, v = inputs(rng, n, n, qh, 1, d, dtype)
+    clean = run(rl, q, k, v, qs, 1, dtype).reshape(q.shape)
+    bad = k8.floats(v, dtype)
+    bad[0, 0, 3], bad[700, 0, 9], bad[700, 0, 11], bad[:, 0, 20] = np.nan, np.nan, -np.inf, np.inf
+    out = run(rl, q, k, k8.bits(bad, dtype), qs, 1, dtype).reshape(q.shape)
+    f = k8.floats(out, dtype)
+    assert np.isnan(f[:, :, 3]).all() and np.isnan(f[700:, :, 9]).all() and np.isneginf(f[700:, :, 11]).all()
+    assert np.isposinf(f[:, :, 20]).all()
+    out[:, :, [3, 20]], out[700:, :, [9, 11]] = clean[:, :, [3, 20]], clean[700:, :, [9, 11]]
+    compare(clean, q, k, v, qs, qs, 1, dtype)
+    compare(out, q, k, v, qs, qs, 1, dtype)
+    # where no row's last tiles hold one, the others keep their bits (in fp16 such rows are computed again)
+    bad = k8.floats(v, dtype)
+    bad[0, 0, 3] = np.nan
+    out = run(rl, q, k, k8.bits(bad, dtype), qs, 1, dtype).reshape(q.shape)
+    assert dtype == "fp16" or np.array_equal(np.delete(out, 3, 2), np.delete(clean, 3, 2))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_infinity_of_little_weight(rl, gpu, dtype):
+    """A seen infinity whose weight, 2^-40 of the largest, fp16 does not hold: the outputs are infinite, not NaN. Whole
+    prompts, and the last queries behind keys that workgroups share."""
+    rng = np.random.default_rng(19)
+    n, d = 900, 64
+    q, k, v = inputs(rng, n, n, 2, 1, d, dtype)
+    fq, fk, fv = (k8.floats(x, dtype) for x in (q, k, v))
+    fq[:] = fk[:] = 0.0
+    fq[:, :, 0], fk[1:, 0, 0] = 8.0, 28.0  # scores 0 for key 0 and 28 (2^40.4) for the others
+    fv[0, 0, 6], fv[0, 0, 7] = np.inf, -np.inf
+    q, k, v = (k8.bits(x, dtype) for x in (fq, fk, fv))
+    f = k8.floats(run(rl, q, k, v, [0, n], 1, dtype).reshape(q.shape), dtype)
+    assert np.isposinf(f[:, :, 6]).all() and np.isneginf(f[:, :, 7]).all() and np.isfinite(np.delete(f, [6, 7], 2)).all()
+    f = k8.floats(run(rl, q[-3:], k, v, [0, 3], 1, dtype, kv_starts=[0, n]).reshape(3, 2, d), dtype)
+    assert np.isposinf(f[:, :, 6]).all() and np.isneginf(f[:, :, 7]).all() and np.isfinite(np.delete(f, [6, 7], 2)).all()
+
+
+@pytest.mark.parametrize("nq, nk", [(3000, 3000), (16, 6000)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_values_that_are_no_numbers_cost_little(rl, gpu, dtype, nq, nk):
+    """A NaN in the first value, and infinities in a dim of all: the call takes a few times as long as without them, not
+    hundreds of times (each of its rows again, key by key)."""
+    d, qh, kvh = 128, 8, 2
+    q, k, v = inputs(np.random.default_rng(23), nq, nk, qh, kvh, d, dtype)
+    up = rl.DeviceBuffer.from_array
+    dev = [up(q), up(k), up(v), up(np.zeros_like(q)), up(np.array([0, nq], np.uint32)), up(np.array([0, nk], np.uint32))]
+    args = rl.AttnPromptArgs(q=dev[0].ptr, k=dev[1].ptr, v=dev[2].ptr, out=dev[3].ptr, q_starts=dev[4].ptr,
+                             kv_starts=dev[5].ptr, seqs=1, q_tokens=nq, kv_tokens=nk, max_q=nq, max_kv=nk, q_heads=qh,
+                             kv_heads=kvh, head_dim=d, dtype=k8.dtype_id(rl, dtype))
+    ws = rl.attn_prompt_workspace(args)
+    timer = rl.Timer()
+
+    def least():
+        times = []
+        for _ in range(6):
+            timer.begin()
+            rl.attn_prompt(args)
+            times.append(timer.end())
+        return min(times)
+
+    clean = least()
+    for rows, what in ((0, np.nan), (slice(None), np.inf)):
+        bad = k8.floats(v, dtype)
+        bad[rows, :, 5] = what
+        dev[2].upload(k8.bits(bad, dtype))
+        assert least() < 12 * clean + 0.1
+    for b in dev + [ws]:
+        b.close()
+
+
 def test_strides_and_bounds(rl, gpu):
     """q, k and v as slices of one row, a wider output whose gaps stay, rows of no sequence left alone, starts past the
     arrays cut off, a sequence longer than max_q."""
