@@ -229,6 +229,19 @@ def test_decode_kernels(rl, gpu, batch, kvh, group, t, d, dtype, max_ctx, lens):
     assert not out32.any() and not out16.any()
 
 
+@pytest.mark.parametrize("kvh", [1, 2])
+@pytest.mark.parametrize("ctx", [[1, 0, 0], [0, 0, 40], [30, 700, 0], [300, 31, 900], [0, 3, 2500]])
+def test_decode_far_below_max_ctx(rl, gpu, ctx, kvh):
+    """Contexts far below max_ctx: fewer runs than XCDs, none on some, and a few more than XCDs."""
+    rng = np.random.default_rng(sum(ctx))
+    for max_ctx in (1 << 20, 20000):  # even shares, and workgroups that own their rows
+        arena, table, q = decode_case(rng, ctx, kvh, 4, 16, 128, "bf16", stride=-(-max_ctx // 16))
+        out16, out32 = k8.run_decode(rl, arena, table, ctx, q, "bf16", max_ctx)
+        check(arena, table, ctx, q, out16, out32, "bf16")
+        again = k8.run_decode(rl, arena, table, ctx, q, "bf16", max_ctx, graph=2)
+        assert np.array_equal(again[1].view(np.uint32), out32.view(np.uint32))
+
+
 def test_decode_bad_rows(rl, gpu):
     """A context past max_ctx and a block past the arena give NaN rows; the others keep their bits. NaN among a row's own
     tokens reaches only the outputs that see it."""

@@ -1,6 +1,7 @@
 """The 8-bit KV cache and the prompt attention without a GPU: layouts, the
 ctypes mirror, and every refusal (the arguments are checked before the device)."""
 import ctypes as C
+from collections import Counter
 
 import numpy as np
 import pytest
@@ -38,6 +39,22 @@ def test_e4m3_model():
     assert np.array_equal(k8.to_e4m3(mid * (1 + 2.0 ** -40)), np.arange(1, 127))
     assert k8.scale_of(np.array([448.0])) == 1 and k8.scale_of(np.array([448.01])) == 2
     assert k8.scale_of(np.array([0.0, np.inf, np.nan])) == k8.LEAST
+
+
+@pytest.mark.parametrize("grid", [512, 64, 16, 510])
+def test_runs_over_the_xcds(grid):
+    """However few of a grid's workgroups have work (workgroup b runs on XCD b % 8): each run once, on all XCDs alike,
+    neighbours on one XCD."""
+    probe = helpers.load_shared("tests/c/kv8_runs_probe.c", link_runtime=False)
+    probe.kv8_probe_run.restype = C.c_uint32
+    for n in [1, 2, 7, 8, 9, grid // 3, grid - 1, grid]:
+        runs = {b: probe.kv8_probe_run(b, grid, n) for b in range(grid)}
+        has = {r: b % 8 for b, r in runs.items() if r != 0xFFFFFFFF}
+        assert sorted(has) == list(range(n)) and sum(r != 0xFFFFFFFF for r in runs.values()) == n
+        per_xcd = [Counter(has.values())[x] for x in range(8)]
+        assert max(per_xcd) - min(per_xcd) <= 1, (n, per_xcd)
+        if grid % 8 == 0:
+            assert [has[r] for r in range(n)] == sorted(has.values())
 
 
 def append_args(rl, **kw):
