@@ -44,8 +44,8 @@
 
 namespace {
 
-constexpr int kUnit = 32;           // tokens per unit
-constexpr uint32_t kRowCost = 8;    // units that turning to a row is worth
+constexpr int kUnit = KV8_UNIT;
+constexpr uint32_t kRowCost = KV8_ROW_COST;
 constexpr uint64_t kKeptBytes = 256u << 20;  // what the last cache before HBM holds
 
 struct Kv8Params {
@@ -447,18 +447,21 @@ __device__ __forceinline__ bool shares_blocks(const Kv8Params &p, uint32_t b, ui
 // workgroups, two per compute unit, take equal runs of it, whatever the
 // contexts are; where these are short of max_ctx and the runs are fewer than the
 // workgroups, they still lie on all XCDs (8 x 500 tokens, max_ctx 32,768: 11.2 us
-// against 13.5 on the first three). A run that covers a row writes its output; a row that several
-// share is merged from their partials. A workgroup has at most two of those, of
-// the rows its run starts and ends in: number 2 w when the row's part starts
-// the run, else 2 w + 1.
-// Where all rows are more than the last cache keeps for a next call, the rows of
-// rollouts that share no prompt with their neighbours are read past the caches:
+// against 13.5 on the first three). A run that covers a row writes its output; a
+// row that several share is merged from their partials. A workgroup has at most
+// two of those, of the rows its run starts and ends in: number 2 w when the row's
+// part starts the run, else 2 w + 1.
+// Where the rows' bytes, those of shared blocks once for each rollout, are more
+// than the last cache keeps for a next call, the rows of rollouts whose first
+// block is not that of the rollout before or after them are read past the caches:
 // 8 x 32,768 tokens (539 MB) 94.5 us against 104, and 109 against 116 behind a
 // product with 1 GiB of weights, as in a model's step; 64 x 512-4,096 (304 MB) 62
-// against 67. What is kept pays below (64 x 1,536 again and again 35.6 against
-// 37.4), with shared prompts (64 x 4,096, three quarters shared by eight, 67
-// against 82), and right behind 1 GiB of writes, which the last cache still has to
-// put away (107 against 140): that last one the kernel cannot see.
+// against 67. What is kept pays below (64 x 1,800 again and again 42.8 against
+// 48.0, 512 x 200 64.8 against 79.1; where three such sets are read in turn 49.6
+// against 46.5 and 75.7 against 81.2), with shared prompts (64 x 4,096, three
+// quarters shared by eight, 67 against 82, also where the eight are not
+// neighbours, which is not looked for), and right behind 1 GiB of writes, which the
+// last cache still has to put away (107 against 140): that the kernel cannot see.
 template <int D, int DT, int TPB, int W>
 __global__ __launch_bounds__(W * 64) void attn_kv8_even_kernel(Kv8Params p)
 {
@@ -469,9 +472,12 @@ __global__ __launch_bounds__(W * 64) void attn_kv8_even_kernel(Kv8Params p)
         return b0 + lane < p.batch ? cost_of(units_of(p, p.ctx[b0 + lane])) * p.kv_heads : 0u;
     };
     const uint32_t t0 = cost64(0);
-    uint32_t total = rl_wave_sum_u32(t0);
-    for (uint32_t b0 = 64; b0 < p.batch; b0 += 64)
-        total += rl_wave_sum_u32(cost64(b0));
+    uint32_t total = rl_wave_sum_u32(t0), filled = (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(t0 != 0));
+    for (uint32_t b0 = 64; b0 < p.batch; b0 += 64) {
+        const uint32_t t = cost64(b0);
+        total += rl_wave_sum_u32(t);
+        filled += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(t != 0));
+    }
     const uint32_t n = sharing(p, total);
     // (the wave, not its threads, decides: what follows stays in scalar registers)
     const uint32_t wg = __builtin_amdgcn_readfirstlane(kv8_run_of(blockIdx.x, gridDim.x, n));
@@ -502,7 +508,7 @@ __global__ __launch_bounds__(W * 64) void attn_kv8_even_kernel(Kv8Params p)
         return;
     uint32_t cin = rl_sload(p.ctx + b), nu = units_of(p, cin);
     uint32_t g = (first - before) / cost_of(nu), x = (first - before) % cost_of(nu);  // x: of this row's cost
-    const bool once = (uint64_t)total * (2 * kUnit * D) > kKeptBytes;
+    const bool once = kv8_bytes_of(total, filled * p.kv_heads, D) > kKeptBytes;
     uint32_t parts = 0;
     for (uint32_t at = first; at < last;) {
         const uint32_t m = min(cost_of(nu) - x, last - at);

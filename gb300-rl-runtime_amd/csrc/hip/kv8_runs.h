@@ -13,6 +13,15 @@
 #endif
 
 #define KV8_NO_RUN UINT32_MAX
+#define KV8_UNIT 32u     // tokens per unit
+#define KV8_ROW_COST 8u  // units that turning to a row is worth
+
+// Bytes of the cache that rows of `cost` units in all hold, `rows` of them not empty:
+// the row costs are nothing that is read.
+KV8_HD uint64_t kv8_bytes_of(uint64_t cost, uint32_t rows, uint32_t head_dim)
+{
+    return (cost - (uint64_t)rows * KV8_ROW_COST) * (2u * KV8_UNIT * head_dim);
+}
 
 // Workgroup `block` of `grid`: a contiguous eighth of the grid's parts per XCD.
 KV8_HD uint32_t kv8_contiguous(uint32_t block, uint32_t grid)

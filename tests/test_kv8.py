@@ -57,6 +57,18 @@ def test_runs_over_the_xcds(grid):
             assert [has[r] for r in range(n)] == sorted(has.values())
 
 
+@pytest.mark.parametrize("rows, tokens, d, past", [(64 * 8, 1800, 128, False), (512 * 8, 200, 128, False), (64 * 8, 2048, 128, False),
+                                                   (64 * 8, 2080, 128, True), (512 * 8, 260, 128, True), (8 * 8, 32768, 64, False),
+                                                   (8 * 8, 32800, 64, True), (0, 0, 128, False)])
+def test_bytes_that_are_read(rows, tokens, d, past):
+    """What is read past the caches is decided by the bytes of the rows, not by what turning to them costs as well."""
+    probe = helpers.load_shared("tests/c/kv8_runs_probe.c", link_runtime=False)
+    probe.kv8_probe_bytes.restype = C.c_uint64
+    units = -(-tokens // 32)
+    got = probe.kv8_probe_bytes(C.c_uint64(rows * (units + 8)), rows, d)
+    assert got == rows * units * 32 * 2 * d and (got > 256 << 20) == past
+
+
 def append_args(rl, **kw):
     a = dict(arena_base=P, arena_bytes=1 << 20, layout=rl.KvLayoutDesc.paged8(16, 128), block_table=P, table_stride=4,
              batch=2, kv_heads=8, dtype=rl.DTYPE_BF16, positions=P, starts=None, tokens=2, max_new=1, cow_src=None,
