@@ -624,6 +624,7 @@ struct Plan8 {
     bool even;
     uint32_t split, min_units, waves;
     size_t part_off, total;  // of the workspace
+    size_t most;             // the largest total of calls up to this one's batch and max_ctx
 };
 
 Plan8 plan_of(const rl_attn_decode_args_t *a)
@@ -648,6 +649,9 @@ Plan8 plan_of(const rl_attn_decode_args_t *a)
     const size_t part = (size_t)(G * a->layout.head_dim + 2 * G) * sizeof(float);
     pl.part_off = pl.even ? (((size_t)a->batch + 1) * 4 + 255) / 256 * 256 : 0;
     pl.total = 256 + pl.part_off + (pl.even ? 2 * (size_t)pl.split * part : pl.split > 1 ? rows * pl.split * part : 0);
+    // no more for any smaller batch and max_ctx: the rows kernel's shares are at most these
+    const uint64_t shares = units < kWholeUnits ? 0 : std::min<uint64_t>(2 * cus, rows * (units / kShareUnits));
+    pl.most = pl.even ? pl.total : 256 + shares * part;
     return pl;
 }
 
@@ -746,7 +750,7 @@ extern "C" size_t rl_hip_attn_decode_kv8_workspace(const rl_attn_decode_args_t *
 {
     if (validate(a, "rl_hip_attn_decode_kv8_workspace") || rl_require_open("rl_hip_attn_decode_kv8_workspace"))
         return 0;
-    return plan_of(a).total;
+    return plan_of(a).most;
 }
 
 extern "C" int rl_hip_attn_decode_kv8(const rl_attn_decode_args_t *a)

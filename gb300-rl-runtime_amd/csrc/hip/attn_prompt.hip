@@ -753,6 +753,7 @@ __global__ __launch_bounds__(256) void attn_prompt_merge_kernel(PromptParams p)
 struct PromptPlan {
     uint32_t tiles, pairs, split;
     size_t workspace;
+    size_t most;  // the largest workspace of calls up to this one's seqs, max_q and max_kv
 };
 
 PromptPlan plan_of(const rl_attn_prompt_args_t *a)
@@ -770,8 +771,13 @@ PromptPlan plan_of(const rl_attn_prompt_args_t *a)
             shares = 2 * cus / blocks;
     }
     pl.split = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(shares, keys / kShareTiles));
-    const size_t part = (size_t)(a->head_dim / 32 * 16 + 2) * 64 * sizeof(float);
-    pl.workspace = 256 + (pl.split > 1 ? (size_t)blocks * pl.split * NW * part : 0);
+    const size_t part = (size_t)NW * (a->head_dim / 32 * 16 + 2) * 64 * sizeof(float);
+    pl.workspace = 256 + (pl.split > 1 ? (size_t)blocks * pl.split * part : 0);
+    // no more for any fewer row blocks and keys: at most one share, or two, per compute unit
+    const uint64_t few = std::min(blocks, cus), each = keys / kShareTiles;
+    pl.most = 256;
+    if (few > 0 && each > 1)
+        pl.most += std::min(keys >= kLongShareTiles * (2 * cus / few) ? 2 * cus : cus, few * each) * part;
     return pl;
 }
 
@@ -861,7 +867,7 @@ extern "C" size_t rl_hip_attn_prompt_workspace(const rl_attn_prompt_args_t *a)
 {
     if (validate(a, "rl_hip_attn_prompt_workspace") || rl_require_open("rl_hip_attn_prompt_workspace"))
         return 0;
-    return plan_of(a).workspace;
+    return plan_of(a).most;
 }
 
 extern "C" int rl_hip_attn_prompt(const rl_attn_prompt_args_t *a)

@@ -167,6 +167,8 @@ typedef struct {
     size_t workspace_bytes;
 } rl_attn_prompt_args_t;
 
+/* Enough also for every call with the same heads, head_dim and at most these
+ * seqs, max_q and max_kv. */
 size_t rl_hip_attn_prompt_workspace(const rl_attn_prompt_args_t *args);
 int rl_hip_attn_prompt(const rl_attn_prompt_args_t *args);
 
@@ -224,6 +226,8 @@ typedef struct {
 
 int rl_hip_kv8_append(const rl_kv8_append_args_t *args);
 
+/* Enough also for every call with the same heads, head_dim and at most this
+ * batch and max_ctx. */
 size_t rl_hip_attn_decode_kv8_workspace(const rl_attn_decode_args_t *args);
 int rl_hip_attn_decode_kv8(const rl_attn_decode_args_t *args);
 

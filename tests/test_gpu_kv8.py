@@ -300,6 +300,43 @@ def test_decode_workspace_refused(rl, gpu):
         assert "workspace" in rl.lib().rl_hip_last_error().decode()
 
 
+@pytest.mark.parametrize("kvh, group, d", [(8, 4, 128), (1, 16, 64), (2, 1, 128)])
+def test_decode_workspace_of_smaller_calls(rl, gpu, kvh, group, d):
+    """A workspace of the largest call is enough for every smaller batch and max_ctx."""
+    def args(batch, max_ctx, **kw):
+        return rl.AttnArgs(arena_base=1 << 20, arena_bytes=1 << 20, layout=rl.KvLayoutDesc.paged8(16, d), block_table=1 << 20,
+                           table_stride=1 << 16, batch=batch, q_heads=kvh * group, kv_heads=kvh, dtype=0, ctx_lens=1 << 20,
+                           max_ctx=max_ctx, q=1 << 20, out=1 << 20, **kw)
+
+    batches = [1, 2, 3, 8, 15, 16, 17, 24, 31, 32, 33, 64, 100, 128, 256, 257, 300, 512, 1024]
+    ctxs = [1, 500, 736, 737, 800, 2048, 3168, 3169, 4096, 16000, 33000, 500000]
+    need = np.array([[rl.attn_kv8_workspace_bytes(args(b, c)) for c in ctxs] for b in batches])
+    assert (np.diff(need, axis=0) >= 0).all() and (np.diff(need, axis=1) >= 0).all() and need[0, 0] > 0
+
+
+def test_decode_batch_shrinks_on_one_workspace(rl, gpu):
+    """A rollout whose members end one after the other, on the workspace of its first step."""
+    rng = np.random.default_rng(40)
+    t, d, kvh, group, dtype, max_ctx, batch = 16, 64, 4, 2, "bf16", 1100, 96
+    ctx = rng.integers(1, max_ctx + 1, batch).tolist()
+    arena, table, q = decode_case(rng, ctx, kvh, group, t, d, dtype, stride=-(-max_ctx // t))
+    up = rl.DeviceBuffer.from_array
+    a, tb, cb, qb = up(arena.bytes), up(table), up(np.asarray(ctx, np.uint32)), up(q)
+    out, out32 = rl.DeviceBuffer(q.size * 2), rl.DeviceBuffer(q.size * 4)
+    ws = None
+    for n in (96, 64, 63, 33, 17, 8, 3, 1):
+        args = rl.attn_args(a, rl.KvLayoutDesc.paged8(t, d), tb, table.shape[2], n, kvh * group, kvh, rl.DTYPE_BF16, cb, max_ctx,
+                            qb, out, out32)
+        ws = ws or rl.attn_kv8_workspace(args)
+        args.workspace, args.workspace_bytes = ws.ptr, ws.nbytes
+        rl.attn_decode_kv8(args)
+        rl.sync()
+        got16, got32 = out.download(np.uint16, q.shape)[:n], out32.download(np.float32, q.shape)[:n]
+        check(arena, table[:n], ctx[:n], q[:n], got16, got32, dtype)
+    for b in (a, tb, cb, qb, out, out32, ws):
+        b.close()
+
+
 def test_far_blocks(rl, gpu):
     """Blocks behind 4 GiB of arena: tokens appended to them and read back by the decode."""
     rng = np.random.default_rng(32)

@@ -400,6 +400,43 @@ def test_workspace_refusal(rl, gpu, short):
         rl.attn_prompt(a)
 
 
+@pytest.mark.parametrize("qh, kvh, d", [(32, 8, 128), (3, 1, 64)])
+def test_workspace_of_smaller_calls(rl, gpu, qh, kvh, d):
+    """A workspace of the largest call is enough for fewer sequences, queries and keys."""
+    def need(seqs, max_q, max_kv):
+        return rl.attn_prompt_workspace_bytes(rl.AttnPromptArgs(
+            q=1 << 20, k=1 << 20, v=1 << 20, out=1 << 20, q_starts=1 << 20, seqs=seqs, q_tokens=4, kv_tokens=4, max_q=max_q,
+            max_kv=max_kv, q_heads=qh, kv_heads=kvh, head_dim=d, dtype=0))
+
+    seqs, qs = [1, 2, 3, 5, 8, 16, 31, 32, 33, 64, 200], [0, 1, 16, 33, 64, 100, 517, 1024, 8192]
+    ks = [0, 64, 383, 384, 700, 768, 769, 3100, 6000, 6144, 12300, 50000, 200000]
+    all_ = np.array([[[need(s, q, k) for k in ks] for q in qs] for s in seqs])
+    assert all((np.diff(all_, axis=i) >= 0).all() for i in range(3)) and all_[0, 0, 0] > 0
+
+
+def test_pieces_on_the_workspace_of_a_prompt(rl, gpu):
+    """A long prompt, then its last queries behind its keys, on the workspace of the first call."""
+    rng = np.random.default_rng(41)
+    n, qh, kvh, d, dtype = 1700, 8, 2, 64, "fp16"
+    q, k, v = inputs(rng, n, n, qh, kvh, d, dtype)
+    up = rl.DeviceBuffer.from_array
+    ws = None
+    for m in (n, 33, 1):
+        dev = [up(q[n - m:]), up(k), up(v), up(np.zeros((m, qh, d), np.uint16)), up(np.array([0, m], np.uint32)),
+               up(np.array([0, n], np.uint32))]
+        args = rl.AttnPromptArgs(q=dev[0].ptr, k=dev[1].ptr, v=dev[2].ptr, out=dev[3].ptr, q_starts=dev[4].ptr,
+                                 kv_starts=dev[5].ptr, seqs=1, q_tokens=m, kv_tokens=n, max_q=m, max_kv=n, q_heads=qh,
+                                 kv_heads=kvh, head_dim=d, dtype=rl.DTYPE_FP16)
+        ws = ws or rl.attn_prompt_workspace(args)
+        args.workspace, args.workspace_bytes = ws.ptr, ws.nbytes
+        rl.attn_prompt(args)
+        rl.sync()
+        compare(dev[3].download(np.uint16, (m, qh, d)), q[n - m:], k, v, [0, m], [0, n], kvh, dtype)
+        for b in dev:
+            b.close()
+    ws.close()
+
+
 def test_nothing_to_do(rl, gpu):
     a = rl.AttnPromptArgs(q=1 << 20, k=1 << 20, v=1 << 20, out=1 << 20, q_starts=1 << 20, seqs=1, q_tokens=0, kv_tokens=0,
                           max_q=0, max_kv=0, q_heads=8, kv_heads=2, head_dim=64, dtype=0, workspace=1 << 20,
