@@ -423,3 +423,21 @@ def test_decode_more_than_the_caches_keep(rl, gpu, t, d, kvh, n, dtype):
     rows = [0, 1, 4, 6, 9, 10, 11, 16, 17]
     check(arena, table[rows], np.array(ctx)[rows], q[rows], out16[rows], out32[rows], dtype)
     assert not out32[5].any()
+
+
+@pytest.mark.parametrize("t, d, kvh, n, dtype", [(16, 128, 8, 8000, "bf16")])
+def test_decode_shared_prompts_apart(rl, gpu, t, d, kvh, n, dtype):
+    """More than 256 MiB of cache whose rollouts share prompts with others that are not their neighbours, and one with the
+    whole of its blocks."""
+    rng = np.random.default_rng(n)
+    ctx = (n + rng.integers(0, 700, 17)).tolist()
+    ctx[8] = ctx[2] = n  # the same blocks and length, other queries
+    arena, table, q = decode_case(rng, ctx, kvh, 2, t, d, dtype)
+    assert 2 * d * kvh * sum(ctx) > 256 << 20
+    shared = n // t // 2
+    for b, other in ((3, 0), (6, 0), (9, 5), (16, 1)):
+        table[b, :, :shared] = table[other, :, :shared]
+    table[8] = table[2]
+    out16, out32 = k8.run_decode(rl, arena, table, ctx, q, dtype, max(ctx))
+    rows = [0, 1, 2, 3, 5, 6, 8, 9, 16]
+    check(arena, table[rows], np.array(ctx)[rows], q[rows], out16[rows], out32[rows], dtype)

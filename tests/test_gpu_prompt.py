@@ -114,6 +114,18 @@ def test_sequences_in_order(rl, gpu, seqs):
     compare(out.reshape(q.shape), q, k, v, qs, qs, 2, "bf16")
 
 
+@pytest.mark.parametrize("max_q", [1024, 1025])
+def test_sequences_in_batch_order(rl, gpu, max_q):
+    """At most 64 sequences, with as many row blocks as they are put in order by length for, and more."""
+    rng = np.random.default_rng(max_q)
+    lens = rng.choice([0, 1, 17, 64, 129], 64)
+    lens[[7, 63]] = 300, 0
+    qs = starts_of(lens.tolist())
+    q, k, v = inputs(rng, qs[-1], qs[-1], 8, 8, 64, "fp16")
+    out = run(rl, q, k, v, qs, 8, "fp16", max_q=max_q)
+    compare(out.reshape(q.shape), q, k, v, qs, qs, 8, "fp16")
+
+
 @pytest.mark.parametrize("seqs, longest", [(130, 9300), (200, 6200), (20, 9300)])
 def test_one_long_among_short(rl, gpu, seqs, longest):
     """More row blocks than half the compute units share the keys of the one long sequence, one or two workgroups each."""
