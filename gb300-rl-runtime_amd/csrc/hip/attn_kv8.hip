@@ -6,7 +6,7 @@
 // with sK(t), sV(t) the scales of token t's block. Bound: the bytes of the
 // cache, 2 head_dim per token and KV head; for few rows the chain context,
 // table, block, MFMA, merge. Measured, bf16, GQA 4, 8 KV heads, d128: 8 x 32,768
-// tokens (539 MB) 94.5 us, 64 x 512-4,096 (304 MB) 62.2 us; 5.8 us of it are there
+// tokens (539 MB) 95.2 us, 64 x 512-4,096 (304 MB) 62.6 us; 5.8 us of it are there
 // for the shortest contexts too. 1 x 517 tokens 8.0 us, 24 x 64-2,048 of d64 11.0 us.
 //
 //  work   a row (rollout, KV head) is ceil(ctx / 32) units of 32 tokens. Few
@@ -454,13 +454,13 @@ __device__ __forceinline__ bool shares_blocks(const Kv8Params &p, uint32_t b, ui
 // Where the rows' bytes, those of shared blocks once for each rollout, are more
 // than the last cache keeps for a next call, the rows of rollouts whose first
 // block is not that of the rollout before or after them are read past the caches:
-// 8 x 32,768 tokens (539 MB) 94.5 us against 104, and 109 against 116 behind a
-// product with 1 GiB of weights, as in a model's step; 64 x 512-4,096 (304 MB) 62
+// 8 x 32,768 tokens (539 MB) 95 us against 104, and 109 against 116 behind a
+// product with 1 GiB of weights, as in a model's step; 64 x 512-4,096 (304 MB) 62.5
 // against 67. What is kept pays below (64 x 1,800 again and again 42.8 against
 // 48.0, 512 x 200 64.8 against 79.1; where three such sets are read in turn 49.6
 // against 46.5 and 75.7 against 81.2), with shared prompts (64 x 4,096, three
-// quarters shared by eight, 67 against 82, also where the eight are not
-// neighbours, which is not looked for), and right behind 1 GiB of writes, which the
+// quarters shared by eight neighbours, 64 to 68 against 82; where the eight lie
+// apart, which is not looked for, 88), and right behind 1 GiB of writes, which the
 // last cache still has to put away (107 against 140): that the kernel cannot see.
 template <int D, int DT, int TPB, int W>
 __global__ __launch_bounds__(W * 64) void attn_kv8_even_kernel(Kv8Params p)

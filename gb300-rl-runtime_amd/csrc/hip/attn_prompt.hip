@@ -6,10 +6,11 @@
 // of a sequence with Lq queries and Lk >= Lq keys (the queries are its last
 // tokens). Bound: the matrix cores from some hundred tokens on, 4 head_dim
 // operations per head and visible pair; K and V come from L2. Measured, bf16,
-// GQA 4, 8 KV heads, d128: 1 x 8,192 tokens 482-494 us, 1,130 TFLOP/s (372 with
-// zeros: the chip's power sets the clock), 64 x 512-1,024 450 us, 713 TFLOP/s (382
+// GQA 4, 8 KV heads, d128: 1 x 8,192 tokens 482 us, 1,140 TFLOP/s (372 with
+// zeros: the chip's power sets the clock), 64 x 512-1,024 446 us, 720 TFLOP/s (382
 // with zeros; 6.8 key tiles per row block, each block with its own start and
-// end), 1 x 517 12.3 us (latency).
+// end), 1 x 517 12.3 us (136 row blocks on 256 compute units, up to nine tiles one
+// after the other).
 //
 //  rows   a workgroup of NW waves takes 32 NW rows of one (sequence, KV head);
 //         row r is query token r / G, head r % G of the group, so that a
@@ -28,8 +29,14 @@
 //         S^T, rounded to 16 bits, is the B operand of
 //  PV     O^T += V^T P^T, whose A operand ds_read_b64_tr_b16 takes from the
 //         row-major V tile in the same token order. P in the inputs' type: its
-//         rounding, 2^-9 of each weight with bf16, is of the order of the
-//         output's own.
+//         rounding, up to 2^-8 of each weight with bf16, is of the order of the
+//         output's own (against 64 bits 2.0e-3 of the output's norm where 32 bits
+//         rounded once have 1.6e-3); in two parts, as the decode kernels keep it,
+//         it would double PV's products.
+//  LDS    a step of a d128 workgroup reads 128 KiB of operands and stores 32 KiB of
+//         tiles: 1,280 cycles at 128 bytes each, against 1,024 of matrix
+//         instructions per wave. 32 rows per wave thus keep the matrix cores below
+//         80%.
 //  softmax online; the maximum a row's weights refer to is raised only when it
 //         is exceeded by more than 2^8, which the fp32 sums and 16-bit weights
 //         hold without loss, so the output is rarely rescaled.
@@ -910,8 +917,10 @@ extern "C" int rl_hip_attn_prompt(const rl_attn_prompt_args_t *a)
     p.by_tiles = divisor_of(p.tiles);
     p.part = (float *)a->workspace;
     p.by_xcd = p.pairs % 8 == 0;
-    // (each workgroup finds its place for itself: 9 of 3-2,047 tokens, d64, 31 us against 37 in
-    // batch order; with many row blocks it costs: 64 of 512-1,024 tokens 446 us against 437)
+    // (each workgroup finds its place for itself. In us, in this order and in batch order, by row blocks:
+    // of 3-2,047 tokens, d64, 1,152 33 / 38, 2,048 44 / 50, 4,096 75 / 81, 6,144 113 / 116, 8,192 144 / 146;
+    // d128, GQA 4, of 3-1,000 tokens 4,096 75 / 78, 8,192 143 / 142, of 3-700 8,448 127 / 123, 11,264
+    // 166 / 162, of 512-1,024 8,192 225 / 224, 16,384 455 / 446)
     p.ranked = p.seqs > 1 && p.seqs <= 64 && (uint64_t)p.pairs * p.tiles <= 4096;
     p.rank_shift = 0;
     while (a->max_kv >> p.rank_shift > 63)
