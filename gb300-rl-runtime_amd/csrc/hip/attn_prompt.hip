@@ -581,21 +581,22 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     if (__builtin_amdgcn_ballot_w64(odd != 0.f && L == L && w_row + (lane & 31) < rows) != 0) {
         // An infinity or NaN in V spoils its whole tile in the matrix product, also
         // for the rows that do not see it (0 times NaN). Below `whole` every row sees
-        // every key, so what came of those tiles is right; the keys from there to
-        // `held` are at most two tiles' and are looked through. Where they hold only
+        // every key, so what came of those tiles is right; the places from there to
+        // `held`, where those past the last key repeat it, are at most two tiles' and
+        // are looked through. Where they hold only
         // numbers the outputs stand. (In fp16 a weight below 2^-25 is rounded to 0, and
         // 0 times a seen infinity is NaN instead: such outputs are computed again too.)
         // 1 x 8,192 tokens, 480-500 us (fp16 520) without any: a NaN in the first token
         // 501 (fp16 4,700), in the last 2,070 (fp16 2,600), an infinity in a dim of every
         // token 3,800 (fp16 4,700); 16 queries behind 6,000 keys 18 without, 28 (fp16 90),
         // 70 (fp16 116), 69 (fp16 115).
-        const uint32_t whole = max(w_least, first * BT), held = min((w_most + BT - 1) / BT * BT, lk);
+        const uint32_t whole = max(w_least, first * BT), held = (w_most + BT - 1) / BT * BT;
         constexpr int E = D / 64;  // dims per lane
         float spoilt = 0.f;
         for (uint32_t j = whole; j < held; j += 8)
 #pragma unroll
             for (uint32_t i = 0; i < 8; i++) {
-                const uint16_t *x = vbase + (uint64_t)min(j + i, held - 1) * p.v_stride + lane * E;
+                const uint16_t *x = vbase + (uint64_t)min(j + i, min(held, lk) - 1) * p.v_stride + lane * E;
 #pragma unroll
                 for (int e = 0; e < E; e++)
                     spoilt = fmaf(from16<DT>(x[e]), 0.f, spoilt);

@@ -243,6 +243,21 @@ def test_values_that_are_no_numbers_early(rl, gpu, dtype, d):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("nq, nk", [(1, 710), (3, 710), (70, 70), (2, 64), (1, 1), (5, 2501)])
+def test_infinity_in_the_last_value(rl, gpu, dtype, nq, nk):
+    """The last key, which a tile may hold more than once, has infinite values: so has the only row that sees it."""
+    q, k, v = inputs(np.random.default_rng(nk), nq, nk, 4, 2, 128, dtype)
+    clean = run(rl, q, k, v, [0, nq], 2, dtype, kv_starts=[0, nk]).reshape(q.shape)
+    bad = k8.floats(v, dtype)
+    bad[-1, 0, 33], bad[-1, 1, 4] = np.inf, -np.inf
+    out = run(rl, q, k, k8.bits(bad, dtype), [0, nq], 2, dtype, kv_starts=[0, nk]).reshape(q.shape)
+    f = k8.floats(out, dtype)
+    assert np.isposinf(f[-1, :2, 33]).all() and np.isneginf(f[-1, 2:, 4]).all()
+    out[-1, :2, 33], out[-1, 2:, 4] = clean[-1, :2, 33], clean[-1, 2:, 4]
+    compare(out, q, k, v, [0, nq], [0, nk], 2, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 def test_infinity_of_little_weight(rl, gpu, dtype):
     """A seen infinity whose weight, 2^-40 of the largest, fp16 does not hold: the outputs are infinite, not NaN. Whole
     prompts, and the last queries behind keys that workgroups share."""
