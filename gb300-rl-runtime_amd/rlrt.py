@@ -250,6 +250,20 @@ class Kv8AppendArgs(C.Structure):
                 ("v_new", C.c_void_p), ("k_stride", C.c_uint32), ("v_stride", C.c_uint32)]
 
 
+ROPE_HALVES, ROPE_NEIGHBOURS = 0, 1
+
+
+class RopeAppendArgs(C.Structure):
+    _fields_ = [("arena_base", C.c_void_p), ("arena_bytes", C.c_uint64), ("layout", KvLayoutDesc),
+                ("block_table", C.c_void_p), ("table_stride", C.c_uint32), ("batch", C.c_uint32),
+                ("q_heads", C.c_uint32), ("kv_heads", C.c_uint32), ("dtype", C.c_uint32), ("positions", C.c_void_p),
+                ("starts", C.c_void_p), ("tokens", C.c_uint32), ("cow_src", C.c_void_p), ("freqs", C.c_void_p),
+                ("rot_dim", C.c_uint32), ("pairing", C.c_uint32), ("q", C.c_void_p), ("q_out", C.c_void_p),
+                ("k_new", C.c_void_p), ("v_new", C.c_void_p), ("k_out", C.c_void_p), ("q_stride", C.c_uint32),
+                ("q_out_stride", C.c_uint32), ("k_stride", C.c_uint32), ("v_stride", C.c_uint32),
+                ("k_out_stride", C.c_uint32)]
+
+
 class ProjArgs(C.Structure):
     _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("logits", C.c_void_p), ("rows", C.c_uint32),
                 ("vocab", C.c_uint32), ("hidden", C.c_uint32), ("x_stride", C.c_uint32),
@@ -366,6 +380,8 @@ def load(path: str = LIB_PATH) -> C.CDLL:
         "rl_hip_kv8_append": (i32, [C.POINTER(Kv8AppendArgs)]),
         "rl_hip_attn_decode_kv8_workspace": (sz, [C.POINTER(AttnArgs)]),
         "rl_hip_attn_decode_kv8": (i32, [C.POINTER(AttnArgs)]),
+        "rl_hip_rope_append": (i32, [C.POINTER(RopeAppendArgs)]),
+        "rl_rope_freqs": (i32, [vp, u32, C.c_double]),
         "rl_hip_logits_proj": (i32, [C.POINTER(ProjArgs)]),
         "rl_hip_reward_advantage": (i32, [C.POINTER(RewardArgs)]),
         "rl_hip_rollout_schedule": (i32, [C.POINTER(SchedArgs)]),
@@ -744,6 +760,18 @@ def attn_kv8_workspace(args: AttnArgs) -> DeviceBuffer:
 def attn_decode_kv8(args: AttnArgs) -> None:
     """attn_decode over an 8-bit arena (layout KvLayoutDesc.paged8)."""
     check(lib().rl_hip_attn_decode_kv8(C.byref(args)), "rl_hip_attn_decode_kv8")
+
+
+def rope_freqs(rot_dim: int, theta: float = 10000.0) -> np.ndarray:
+    """theta^(-2 i / rot_dim): radians per position of each pair."""
+    freqs = np.empty(rot_dim // 2, np.float64)
+    check(lib().rl_rope_freqs(ptr(freqs), rot_dim, theta), "rl_rope_freqs")
+    return freqs
+
+
+def rope_append(args: RopeAppendArgs) -> None:
+    """Queries and keys turned by their positions, keys and values into the 16-bit arena."""
+    check(lib().rl_hip_rope_append(C.byref(args)), "rl_hip_rope_append")
 
 
 def kv_append(args: AppendArgs) -> None:

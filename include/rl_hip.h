@@ -172,6 +172,64 @@ typedef struct {
 size_t rl_hip_attn_prompt_workspace(const rl_attn_prompt_args_t *args);
 int rl_hip_attn_prompt(const rl_attn_prompt_args_t *args);
 
+/* ---- positions and the 16-bit cache -------------------------------------------
+ * No reference function (its queries and cache rows come as they are). Turns
+ * the queries and keys of new tokens by their positions and appends keys and
+ * values to the arena in one launch: row b's new tokens are the rows starts[b]
+ * .. starts[b + 1] - 1 of q, k_new and v_new (row b alone when starts is NULL),
+ * at positions[b], positions[b] + 1, ... Of each query and key head the first
+ * rot_dim elements are turned in pairs, (x, y) -> (x cos t - y sin t, x sin t + y
+ * cos t) with t = position * freqs[i] for pair i: the elements i and i + rot_dim
+ * / 2 (RL_ROPE_HALVES) or 2 i and 2 i + 1 (RL_ROPE_NEIGHBOURS). t is formed in
+ * 64 bits, the products in 32, and each result is rounded once; other elements
+ * and the values keep their bits. rl_rope_freqs fills theta^(-2 i / rot_dim); any
+ * other frequencies (stretched ones for long contexts) do as well.
+ *
+ * q_out may be q with the same stride; otherwise outputs and inputs may not
+ * overlap. k_out takes the turned keys as rows too, for rl_hip_attn_prompt or
+ * rl_hip_kv8_append, with or without an arena. With cow_src[b * kv_heads + g]
+ * >= 0 the slots before row b's first new token are first taken from that
+ * (shared) block of the arena, as in rl_hip_kv_append; no row may write a block
+ * that another row of the call copies from, and no two rows the same block.
+ * Positions past the block table and blocks past arena_bytes are not written
+ * (queries and k_out are); rows of q that belong to no row of the batch leave
+ * q_out and k_out as they were. */
+#define RL_ROPE_HALVES 0u
+#define RL_ROPE_NEIGHBOURS 1u
+typedef struct {
+    void *arena_base;            /* device, 16-byte aligned, or NULL: nothing is appended */
+    uint64_t arena_bytes;        /* blocks past it are never read or written */
+    KvLayoutDesc layout;         /* must pass kv_layout_check_paged (head_dim also without an arena) */
+    const uint32_t *block_table; /* device [batch][kv_heads][table_stride] */
+    uint32_t table_stride;
+    uint32_t batch;              /* 1 .. 65,535 */
+    uint32_t q_heads;
+    uint32_t kv_heads;
+    uint32_t dtype;              /* RL_DTYPE_* of q, K and V */
+    const uint32_t *positions;   /* device [batch]: of each row's first new token */
+    const uint32_t *starts;      /* device [batch + 1], not decreasing, or NULL: one token per row */
+    uint32_t tokens;             /* rows of q, k_new and v_new (batch without starts), below 2^31 */
+    const int32_t *cow_src;      /* device [batch][kv_heads] or NULL */
+    const double *freqs;         /* device [rot_dim / 2]: radians per position */
+    uint32_t rot_dim;            /* a multiple of 16 up to head_dim; 0: nothing is turned */
+    uint32_t pairing;            /* RL_ROPE_* */
+    const void *q;               /* device [tokens][q_heads][head_dim] or NULL: no queries */
+    void *q_out;                 /* device, same shape */
+    const void *k_new;           /* device [tokens][kv_heads][head_dim] */
+    const void *v_new;           /* device [tokens][kv_heads][head_dim]; not read without an arena */
+    void *k_out;                 /* device [tokens][kv_heads][head_dim] or NULL */
+    uint32_t q_stride;           /* elements between tokens: 0 (no gap) or a multiple of 8 */
+    uint32_t q_out_stride;
+    uint32_t k_stride;
+    uint32_t v_stride;
+    uint32_t k_out_stride;
+} rl_rope_append_args_t;
+
+int rl_hip_rope_append(const rl_rope_append_args_t *args);
+/* Host: freqs[i] = theta^(-2 i / rot_dim), i < rot_dim / 2. -1 for a NULL
+ * pointer, an odd rot_dim or a theta that is not positive. */
+int rl_rope_freqs(double *freqs, uint32_t rot_dim, double theta);
+
 /* ---- the 8-bit KV cache -------------------------------------------------------
  * No reference function (its cache is 2-byte scalars). An arena whose layout
  * is kv_layout_desc_paged8: e4m3 blocks, each plane (K, V) with one
