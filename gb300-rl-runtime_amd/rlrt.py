@@ -264,6 +264,15 @@ class RopeAppendArgs(C.Structure):
                 ("k_out_stride", C.c_uint32)]
 
 
+class AttnChunkArgs(C.Structure):
+    _fields_ = [("arena_base", C.c_void_p), ("arena_bytes", C.c_uint64), ("layout", KvLayoutDesc),
+                ("block_table", C.c_void_p), ("table_stride", C.c_uint32), ("batch", C.c_uint32),
+                ("q_heads", C.c_uint32), ("kv_heads", C.c_uint32), ("dtype", C.c_uint32), ("ctx_lens", C.c_void_p),
+                ("max_ctx", C.c_uint32), ("q_starts", C.c_void_p), ("q_tokens", C.c_uint32), ("max_q", C.c_uint32),
+                ("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_uint32), ("out_stride", C.c_uint32),
+                ("scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 class ProjArgs(C.Structure):
     _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("logits", C.c_void_p), ("rows", C.c_uint32),
                 ("vocab", C.c_uint32), ("hidden", C.c_uint32), ("x_stride", C.c_uint32),
@@ -381,6 +390,8 @@ def load(path: str = LIB_PATH) -> C.CDLL:
         "rl_hip_attn_decode_kv8_workspace": (sz, [C.POINTER(AttnArgs)]),
         "rl_hip_attn_decode_kv8": (i32, [C.POINTER(AttnArgs)]),
         "rl_hip_rope_append": (i32, [C.POINTER(RopeAppendArgs)]),
+        "rl_hip_attn_chunk_workspace": (sz, [C.POINTER(AttnChunkArgs)]),
+        "rl_hip_attn_chunk": (i32, [C.POINTER(AttnChunkArgs)]),
         "rl_rope_freqs": (i32, [vp, u32, C.c_double]),
         "rl_hip_logits_proj": (i32, [C.POINTER(ProjArgs)]),
         "rl_hip_reward_advantage": (i32, [C.POINTER(RewardArgs)]),
@@ -737,6 +748,24 @@ def attn_prompt_workspace(args: AttnPromptArgs) -> DeviceBuffer:
 def attn_prompt(args: AttnPromptArgs) -> None:
     """Causal attention over packed whole prompts."""
     check(lib().rl_hip_attn_prompt(C.byref(args)), "rl_hip_attn_prompt")
+
+
+def attn_chunk_workspace_bytes(args: AttnChunkArgs) -> int:
+    n = lib().rl_hip_attn_chunk_workspace(C.byref(args))
+    if n == 0:
+        raise RlrtError(f"rl_hip_attn_chunk_workspace: {_err()}")
+    return int(n)
+
+
+def attn_chunk_workspace(args: AttnChunkArgs) -> DeviceBuffer:
+    ws = DeviceBuffer(attn_chunk_workspace_bytes(args))
+    args.workspace, args.workspace_bytes = ws.ptr, ws.nbytes
+    return ws
+
+
+def attn_chunk(args: AttnChunkArgs) -> None:
+    """Causal attention of each row's newest tokens over the 16-bit arena."""
+    check(lib().rl_hip_attn_chunk(C.byref(args)), "rl_hip_attn_chunk")
 
 
 def kv8_append(args: Kv8AppendArgs) -> None:

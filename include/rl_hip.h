@@ -230,6 +230,48 @@ int rl_hip_rope_append(const rl_rope_append_args_t *args);
  * pointer, an odd rot_dim or a theta that is not positive. */
 int rl_rope_freqs(double *freqs, uint32_t rot_dim, double theta);
 
+/* ---- attention of chunks over the 16-bit cache --------------------------------
+ * No reference function (its worker decodes single tokens). Causal attention
+ * of each rollout's newest tokens over the arena blocks that hold all of its
+ * tokens, those included (append them first): row b's queries are q_starts[b] ..
+ * q_starts[b + 1] - 1, its keys and values the tokens 0 .. ctx_lens[b] - 1 behind
+ * its block table, as in rl_hip_attn_decode. The queries are the last tokens:
+ * query i of Lq sees the keys j <= i + ctx_lens[b] - Lq. One token per row is a
+ * decode step; more are a piece of a prompt, or drafted tokens to be checked.
+ * Heads, sums and rounding, queries that see no key, values that are no numbers
+ * and rows of out that belong to no sequence are as in rl_hip_attn_prompt. A row
+ * whose context exceeds max_ctx gets NaN outputs, and so does every query that
+ * sees a key of a block past arena_bytes (which is not read). */
+typedef struct {
+    const void *arena_base;      /* device, 16-byte aligned */
+    uint64_t arena_bytes;        /* blocks past it are never read */
+    KvLayoutDesc layout;         /* must pass kv_layout_check_paged */
+    const uint32_t *block_table; /* device [batch][kv_heads][table_stride] */
+    uint32_t table_stride;
+    uint32_t batch;              /* 1 .. 65,535 */
+    uint32_t q_heads;
+    uint32_t kv_heads;           /* divides q_heads */
+    uint32_t dtype;              /* RL_DTYPE_* of q, K, V and out */
+    const uint32_t *ctx_lens;    /* device [batch]: tokens in the cache */
+    uint32_t max_ctx;            /* upper bound of ctx_lens, at most table_stride blocks */
+    const uint32_t *q_starts;    /* device [batch + 1], not decreasing */
+    uint32_t q_tokens;           /* rows of q and out; below 2^31 */
+    uint32_t max_q;              /* upper bound of a row's queries; later ones get no output. */
+                                 /* batch * kv_heads * ceil(max_q * q_heads / kv_heads / 128) < 2^24 */
+    const void *q;               /* device [q_tokens][q_heads][head_dim], tokens q_stride elements apart */
+    void *out;                   /* device [q_tokens][q_heads][head_dim]; may not overlap the inputs */
+    uint32_t q_stride;           /* elements; 0: no gap. Else a multiple of 8, at least a token's own, at most 2^24 */
+    uint32_t out_stride;
+    float scale;                 /* positive; 0 selects 1/sqrt(head_dim) */
+    void *workspace;             /* device, >= rl_hip_attn_chunk_workspace() */
+    size_t workspace_bytes;
+} rl_attn_chunk_args_t;
+
+/* Enough also for every call with the same heads, head_dim and at most this
+ * batch, max_q and max_ctx. */
+size_t rl_hip_attn_chunk_workspace(const rl_attn_chunk_args_t *args);
+int rl_hip_attn_chunk(const rl_attn_chunk_args_t *args);
+
 /* ---- the 8-bit KV cache -------------------------------------------------------
  * No reference function (its cache is 2-byte scalars). An arena whose layout
  * is kv_layout_desc_paged8: e4m3 blocks, each plane (K, V) with one
