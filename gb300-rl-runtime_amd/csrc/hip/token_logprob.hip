@@ -1,0 +1,610 @@
+// token_logprob.hip - log probabilities of given tokens under a vocabulary
+// projection, and their gradients, without keeping the logits, on gfx950.
+//
+//   z[r][v] = scale x_r . w_v      lse_r = log sum_v exp z[r][v]      logprob_r = z[r][t_r] - lse_r
+//   D[r][v] = scale g_r (1[v = t_r] - exp(z[r][v] - lse_r))           dx = D w      dw = D^T x
+//
+//  forward   the product's tiles (gemm_core.h) end in each row's maximum and sum
+//            of exponentials over a wave's columns; a second launch joins them.
+//  gradient  in pieces of the vocabulary, of which D (bf16) takes up to 256 MiB:
+//            the logits of the piece again, from them D, then its shares of dx and
+//            its rows of dw, both products of D. dx is summed in fp32 over pieces,
+//            and over shares of a piece's vocabulary where its tiles are few.
+//            D's rounding, up to 2^-9 of each element, is of the order of the
+//            outputs' own.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "gemm_core.h"
+#include "rl_hip.h"
+#include "rl_hip_internal.h"
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// The larger (the sum) of lanes l and l ^ 32, in both.
+__device__ __forceinline__ float pair_max(float x)
+{
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+}
+__device__ __forceinline__ float pair_sum(float x)
+{
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(h[0]) + __uint_as_float(h[1]);
+}
+
+struct LogitParams {
+    GemmOperand w, x;        // w: the piece's rows
+    const uint32_t *targets;
+    float scale;
+    uint32_t rows, vocab, v0;  // v0: the piece's first entry; vocab: of all
+    uint32_t m_tiles, n_tiles;
+    // statistics
+    rl_f32x2 *part;          // [n_tiles * WN][rows]: maximum and sum
+    float *hit;              // [rows]: the target's logit
+    // gradient
+    const float *lse, *grad;
+    uint16_t *d;             // [rows_pad][pitch]
+    uint32_t rows_pad;
+    uint64_t pitch;
+};
+
+template <typename G, bool ROT>
+__device__ __forceinline__ bool logits_of(const LogitParams &p, uint8_t *smem, typename G::Acc &acc, uint32_t &m0,
+                                          uint32_t &nt)
+{
+    uint32_t mt;
+    if (!gemm_tile_of(blockIdx.x, p.m_tiles, p.n_tiles, mt, nt))
+        return false;
+    m0 = mt * G::BM;
+    const uint32_t steps = p.x.k / kGemmK;
+    // Each workgroup starts at another k: all starting at 0, they would read the same columns of rows that lie a
+    // power of two apart together.
+    G::run(p.w, p.x, nt * G::BN, m0, 0, steps, ROT ? blockIdx.x / 8 * 5u % steps : 0u, smem, acc);
+    return true;
+}
+
+template <typename G, bool ROT>
+__global__ __launch_bounds__(G::WAVES * 64) void token_stats_kernel(LogitParams p)
+{
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[G::LDS];
+    typename G::Acc acc;
+    uint32_t m0, nt;
+    if (!logits_of<G, ROT>(p, smem, acc, m0, nt))
+        return;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hf = lane >> 5;
+    const uint32_t wn = wave % G::WN, wm = wave / G::WN, n0 = nt * G::BN + wn * G::TN * 32;
+    const bool whole = n0 + G::TN * 32 <= p.vocab;
+#pragma unroll
+    for (int b = 0; b < G::TM; b++) {
+        const uint32_t row = m0 + (wm * G::TM + b) * 32 + (lane & 31);
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int a = 0; a < G::TN; a++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                float z = acc[a][b][r] * p.scale;
+                if (!whole && n0 + 32 * a + 8 * (r / 4) + 4 * hf + r % 4 >= p.vocab)
+                    z = -INFINITY;
+                acc[a][b][r] = z;
+                top = fmaxf(top, z);
+            }
+        top = pair_max(top);
+        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int a = 0; a < G::TN; a++)
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                sum += __builtin_amdgcn_exp2f((acc[a][b][r] - ref) * kLog2e);
+        sum = pair_sum(sum);
+        if (row < p.rows) {
+            if (hf == 0)
+                p.part[(uint64_t)(nt * G::WN + wn) * p.rows + row] = rl_f32x2{top, sum};
+            const uint32_t t = p.targets[row], at = t - n0;
+            if (t < p.vocab && at < G::TN * 32 && (at >> 2 & 1) == hf) {
+#pragma unroll
+                for (int a = 0; a < G::TN; a++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (at == 32u * a + 8 * (r / 4) + 4 * hf + r % 4)
+                            p.hit[row] = acc[a][b][r];
+            }
+        }
+    }
+}
+
+// Joins the statistics of 16 rows: 16 threads a row, four shares at a time each.
+__global__ __launch_bounds__(256) void token_logprob_kernel(const rl_f32x2 *part, const float *hit,
+                                                            const uint32_t *targets, uint32_t rows, uint32_t vocab,
+                                                            uint32_t slots, float *logprob, float *lse)
+{
+    __shared__ rl_f32x2 all[16][16];
+    const uint32_t r = threadIdx.x % 16, y = threadIdx.x / 16, row = blockIdx.x * 16 + r, at = min(row, rows - 1);
+    float top = -INFINITY, sum = 0.f;
+    auto join = [&](float m, float l) {
+        // (before a maximum, a sum is 0 or no number)
+        const float t = fmaxf(top, m);
+        sum = sum * (top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top - t) * kLog2e)) +
+              l * (m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - t) * kLog2e));
+        top = t;
+    };
+    for (uint32_t s = y; s < slots; s += 64) {
+        rl_f32x2 x[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++)
+            x[i] = part[(uint64_t)min(s + 16 * i, slots - 1) * rows + at];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++)
+            if (s + 16 * i < slots)
+                join(x[i][0], x[i][1]);
+    }
+    all[y][r] = rl_f32x2{top, sum};
+    __syncthreads();
+    if (y != 0 || row >= rows)
+        return;
+    for (uint32_t i = 1; i < 16; i++)
+        join(all[i][r][0], all[i][r][1]);
+    const float z = top == -INFINITY && sum == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + logf(sum);
+    lse[row] = z;
+    logprob[row] = targets[row] < vocab ? hit[row] - z : 0.f;
+}
+
+template <typename G, bool ROT>
+__global__ __launch_bounds__(G::WAVES * 64) void token_delta_kernel(LogitParams p)
+{
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[G::LDS];
+    typename G::Acc acc;
+    uint32_t m0, nt;
+    if (!logits_of<G, ROT>(p, smem, acc, m0, nt))
+        return;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hf = lane >> 5;
+    const uint32_t wn = wave % G::WN, wm = wave / G::WN, n0 = nt * G::BN + wn * G::TN * 32;
+    const bool whole = p.v0 + n0 + G::TN * 32 <= p.vocab;
+#pragma unroll
+    for (int b = 0; b < G::TM; b++) {
+        const uint32_t row = m0 + (wm * G::TM + b) * 32 + (lane & 31);
+        const uint32_t t = row < p.rows ? p.targets[row] : 0xFFFFFFFFu;
+        const bool has = t < p.vocab;  // rows without a target: zeros, whatever their logits are
+        const float g = has ? p.grad[row] * p.scale : 0.f, lse = has ? p.lse[row] : 0.f;
+        const uint32_t at = has ? t - p.v0 - n0 : 0xFFFFFFFFu;
+#pragma unroll
+        for (int a = 0; a < G::TN; a++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const uint32_t n = 32u * a + 8 * (r / 4) + 4 * hf + r % 4;
+                const float e = __builtin_amdgcn_exp2f((acc[a][b][r] * p.scale - lse) * kLog2e);
+                const float x = g * ((n == at ? 1.f : 0.f) - e);
+                acc[a][b][r] = !has || (!whole && p.v0 + n0 + n >= p.vocab) ? 0.f : x;
+            }
+    }
+    uint16_t *d = p.d + nt * G::BN;
+    G::each8(acc, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
+        if (m0 + m < p.rows_pad)
+            *(rl_u32x4 *)(d + (uint64_t)(m0 + m) * p.pitch + n) = w;
+        if (G::BM == 32)  // (rows_pad is 64)
+            *(rl_u32x4 *)(d + (uint64_t)(m + 32) * p.pitch + n) = rl_u32x4{0, 0, 0, 0};
+    });
+}
+
+// x with zeros for the rows without a target and those up to rows_pad, which D's zeros alone would not keep out where they
+// are no numbers. A workgroup copies a row at a time.
+__global__ __launch_bounds__(256) void token_rows_kernel(const uint16_t *x, uint64_t ld, const uint32_t *targets,
+                                                         uint32_t rows, uint32_t rows_pad, uint32_t vocab,
+                                                         uint32_t hidden, uint16_t *out)
+{
+    for (uint32_t row = blockIdx.x; row < rows_pad; row += gridDim.x) {
+        const bool has = row < rows && targets[row] < vocab;
+        for (uint32_t c = threadIdx.x; c < hidden / 8; c += 256)
+            *(rl_u32x4 *)(out + (uint64_t)row * hidden + c * 8) =
+                has ? *(const rl_u32x4 *)(x + row * ld + c * 8) : rl_u32x4{0, 0, 0, 0};
+    }
+}
+
+struct DxParams {
+    GemmOperand w, d;
+    const uint32_t *targets;
+    uint32_t rows, vocab, hidden;
+    uint32_t m_tiles, n_tiles, steps, split;
+    uint32_t add;     // to what an earlier piece left in part
+    float *part;      // [split][rows][hidden], or NULL: to dx
+    uint16_t *dx;
+    uint64_t dx_ld;
+};
+
+template <typename G>
+__global__ __launch_bounds__(G::WAVES * 64) void token_dx_kernel(DxParams p)
+{
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[G::LDS];
+    uint32_t mt, nt;
+    if (!gemm_tile_of(blockIdx.x, p.m_tiles, p.n_tiles, mt, nt))
+        return;
+    const uint32_t m0 = mt * G::BM, n0 = nt * G::BN, share = blockIdx.y;
+    const uint32_t k0 = (uint32_t)((uint64_t)share * p.steps / p.split);
+    const uint32_t k1 = (uint32_t)((uint64_t)(share + 1) * p.steps / p.split);
+    typename G::Acc acc;
+    G::run(p.w, p.d, n0, m0, k0, k1, 0, smem, acc);
+    if (p.part) {
+        float *part = p.part + (uint64_t)share * p.rows * p.hidden;
+        G::each4(acc, [&](uint32_t m, uint32_t n, rl_f32x4 x) {
+            if (m0 + m < p.rows && n0 + n < p.hidden) {
+                float *at = part + (uint64_t)(m0 + m) * p.hidden + n0 + n;
+                if (p.add) {
+                    const rl_f32x4 y = *(const rl_f32x4 *)at;
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        x[e] += y[e];
+                }
+                *(rl_f32x4 *)at = x;
+            }
+        });
+        return;
+    }
+    G::each8(acc, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
+        if (m0 + m < p.rows && n0 + n < p.hidden) {
+            if (p.targets[m0 + m] >= p.vocab)
+                w = rl_u32x4{0, 0, 0, 0};
+            *(rl_u32x4 *)(p.dx + (m0 + m) * p.dx_ld + n0 + n) = w;
+        }
+    });
+}
+
+// dx from its shares, a workgroup a row at a time.
+__global__ __launch_bounds__(256) void token_dx_sum_kernel(DxParams p)
+{
+    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x)
+        for (uint32_t c = threadIdx.x; c < p.hidden / 4; c += 256) {
+            rl_f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            const float *at = p.part + (uint64_t)row * p.hidden + c * 4;
+            for (uint32_t s = 0; s < p.split; s++) {
+                const rl_f32x4 y = *(const rl_f32x4 *)(at + (uint64_t)s * p.rows * p.hidden);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    x[e] += y[e];
+            }
+            rl_u32x2 w = {(uint32_t)to16<0>(x[0]) | (uint32_t)to16<0>(x[1]) << 16,
+                          (uint32_t)to16<0>(x[2]) | (uint32_t)to16<0>(x[3]) << 16};
+            if (p.targets[row] >= p.vocab)
+                w = rl_u32x2{0, 0};
+            *(rl_u32x2 *)(p.dx + row * p.dx_ld + c * 4) = w;
+        }
+}
+
+struct DwParams {
+    GemmOperand x, d;
+    uint32_t entries, hidden;  // of the piece
+    uint32_t m_tiles, n_tiles, steps;
+    uint16_t *dw;
+    uint64_t dw_ld;
+};
+
+template <typename G>
+__global__ __launch_bounds__(G::WAVES * 64) void token_dw_kernel(DwParams p)
+{
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[G::LDS];
+    uint32_t mt, nt;
+    if (!gemm_tile_of(blockIdx.x, p.m_tiles, p.n_tiles, mt, nt))
+        return;
+    const uint32_t m0 = mt * G::BM, n0 = nt * G::BN;
+    typename G::Acc acc;
+    G::run(p.x, p.d, n0, m0, 0, p.steps, 0, smem, acc);
+    G::each8(acc, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
+        if (m0 + m < p.entries && n0 + n < p.hidden)
+            *(rl_u32x4 *)(p.dw + (m0 + m) * p.dw_ld + n0 + n) = w;
+    });
+}
+
+// ---- the host's side ----------------------------------------------------------------
+// Tiles by the number of rows (n along the vocabulary x m along the rows).
+using Rows32 = Gemm<1, 2, 1, 1, 4, false, false>;    // 64 x 32
+using Rows64 = Gemm<1, 2, 2, 1, 4, false, false>;    // 64 x 64
+using Rows128 = Gemm<1, 4, 2, 2, 4, false, false>;   // 128 x 128
+using Rows256 = Gemm<2, 2, 2, 4, 3, false, false>;   // 128 x 256
+using RowsMany = Gemm<4, 2, 2, 4, 2, false, false>;  // 256 x 256
+// (n along hidden)
+using Dx32 = Gemm<1, 4, 1, 1, 4, true, false>;       // 128 x 32
+using Dx64 = Gemm<1, 4, 2, 1, 3, true, false>;       // 128 x 64
+using Dx128 = Gemm<1, 4, 2, 2, 4, true, false>;      // 128 x 128
+using DxMany = Gemm<4, 2, 2, 4, 2, true, false>;     // 256 x 256
+// (n along hidden, m along the vocabulary)
+using Dw = Gemm<4, 2, 2, 4, 2, true, true>;          // 256 x 256
+
+uint32_t tiles_of(uint64_t n, uint32_t per) { return (uint32_t)((n + per - 1) / per); }
+uint32_t grid_of(uint32_t tiles) { return (tiles + 7) / 8 * 8; }
+
+template <typename G>
+uint32_t slots_of(uint32_t vocab) { return tiles_of(vocab, G::BN) * G::WN; }
+
+uint32_t slots_of(uint32_t rows, uint32_t vocab)
+{
+    return rows <= 32    ? slots_of<Rows32>(vocab)
+           : rows <= 64  ? slots_of<Rows64>(vocab)
+           : rows <= 128 ? slots_of<Rows128>(vocab)
+           : rows <= 256 ? slots_of<Rows256>(vocab)
+                         : slots_of<RowsMany>(vocab);
+}
+
+template <typename G, bool ROT>
+int launch_stats(LogitParams p)
+{
+    p.m_tiles = tiles_of(p.rows, G::BM);
+    p.n_tiles = tiles_of(p.w.rows, G::BN);
+    hipLaunchKernelGGL((token_stats_kernel<G, ROT>), dim3(grid_of(p.m_tiles * p.n_tiles)), dim3(G::WAVES * 64), 0,
+                       rl_stream(), p);
+    return rl_check_launch("token_stats_kernel launch");
+}
+
+template <typename G, bool ROT>
+int launch_delta(LogitParams p)
+{
+    p.m_tiles = tiles_of(p.rows, G::BM);
+    p.n_tiles = tiles_of(p.w.rows, G::BN);
+    hipLaunchKernelGGL((token_delta_kernel<G, ROT>), dim3(grid_of(p.m_tiles * p.n_tiles)), dim3(G::WAVES * 64), 0,
+                       rl_stream(), p);
+    return rl_check_launch("token_delta_kernel launch");
+}
+
+template <typename G>
+int launch_dx(DxParams p)
+{
+    p.m_tiles = tiles_of(p.rows, G::BM);
+    p.n_tiles = tiles_of(p.hidden, G::BN);
+    hipLaunchKernelGGL(token_dx_kernel<G>, dim3(grid_of(p.m_tiles * p.n_tiles), p.split), dim3(G::WAVES * 64), 0,
+                       rl_stream(), p);
+    return rl_check_launch("token_dx_kernel launch");
+}
+
+struct GradPlan {
+    uint32_t rows_pad, width;  // rows of D, and its columns: entries of a piece, a multiple of 256
+    uint32_t split;            // shares of a piece's vocabulary for dx
+    bool direct;               // dx from the product itself
+    size_t d, x, part;         // bytes of the workspace's parts
+    size_t most;               // the largest workspace of calls up to this one's rows, vocab and hidden
+};
+
+constexpr uint64_t kDeltaElements = 1ull << 27;  // of D, unless a piece of 1,024 entries has more
+
+// tiles of dx along rows and hidden, and workgroups that run at a time
+template <typename G>
+void dx_shape(uint32_t rows, uint32_t hidden, uint32_t per_cu, uint32_t &tiles, uint32_t &at_once)
+{
+    tiles = tiles_of(rows, G::BM) * tiles_of(hidden, G::BN);
+    at_once = per_cu * rl_cu_count();
+}
+
+size_t up256(uint64_t n) { return (size_t)((n + 255) / 256 * 256); }
+
+GradPlan plan_of(uint32_t rows, uint32_t vocab, uint32_t hidden)
+{
+    GradPlan pl;
+    pl.rows_pad = tiles_of(rows, 64) * 64;
+    const uint32_t all = tiles_of(vocab, 256) * 256;
+    pl.width = std::min(all, std::max<uint32_t>(1024, (uint32_t)(kDeltaElements / pl.rows_pad) / 256 * 256));
+    uint32_t tiles, at_once;
+    if (rows <= 32)
+        dx_shape<Dx32>(rows, hidden, 2, tiles, at_once);
+    else if (rows <= 64)
+        dx_shape<Dx64>(rows, hidden, 2, tiles, at_once);
+    else if (rows <= 128)
+        dx_shape<Dx128>(rows, hidden, 1, tiles, at_once);
+    else
+        dx_shape<DxMany>(rows, hidden, 1, tiles, at_once);
+    // shares of eight steps at least, of the last piece too
+    const uint32_t last = vocab % pl.width ? vocab % pl.width : std::min(pl.width, vocab);
+    pl.split = std::max(1u, std::min(at_once / tiles, last / kGemmK / 8));
+    pl.direct = pl.split == 1 && pl.width >= vocab;
+    pl.d = up256((uint64_t)pl.rows_pad * pl.width * 2);
+    pl.x = up256((uint64_t)pl.rows_pad * hidden * 2);
+    pl.part = pl.direct ? 0 : up256((uint64_t)pl.split * rows * hidden * 4);
+    // D's bound, and as many sums as there are in all tiles at once, or rows
+    const uint64_t d = std::min<uint64_t>((uint64_t)pl.rows_pad * all, std::max<uint64_t>(kDeltaElements, (uint64_t)pl.rows_pad * 1024));
+    const uint64_t at_most = (uint64_t)rl_cu_count() * (rows <= 128 ? 128 * 128 : 256 * 256);
+    pl.most = up256(2 * d) + pl.x + up256(4 * std::max<uint64_t>((uint64_t)rows * hidden, at_most));
+    return pl;
+}
+
+// What both calls have to have.
+int validate(const char *who, const void *x, const void *w, const void *targets, uint32_t rows, uint32_t vocab, uint32_t hidden,
+             uint32_t x_stride, uint32_t w_stride, float scale)
+{
+    if (!x || !w || !targets) {
+        rl_set_error("%s: NULL argument", who);
+        return -1;
+    }
+    if (rows == 0 || rows > (1u << 20) || vocab == 0 || vocab > (1u << 24) || hidden == 0 || hidden % kGemmK != 0 ||
+        hidden > (1u << 16)) {
+        rl_set_error("%s: rows %u (1 to 2^20), vocab %u (1 to 2^24), hidden %u (a multiple of %d up to 2^16)", who, rows,
+                     vocab, hidden, kGemmK);
+        return -1;
+    }
+    // (a launch holds less than 2^32 work-items, 512 for each tile of 256 x 256)
+    if ((uint64_t)((rows + 255) / 256) * ((vocab + 255) / 256) >= (1u << 23) - 8) {
+        rl_set_error("%s: rows %u x vocab %u exceed 2^23 tiles of 256 x 256", who, rows, vocab);
+        return -1;
+    }
+    if (x_stride < hidden || w_stride < hidden || x_stride % 8 != 0 || w_stride % 8 != 0 || x_stride > (1u << 22) ||
+        w_stride > (1u << 22)) {
+        rl_set_error("%s: strides x %u w %u (multiples of 8 from hidden to 2^22)", who, x_stride, w_stride);
+        return -1;
+    }
+    if (!(scale >= 0.f) || std::isinf(scale)) {
+        rl_set_error("%s: scale %g (positive, or 0 for 1)", who, (double)scale);
+        return -1;
+    }
+    if (((uintptr_t)x | (uintptr_t)w) % 16 != 0) {
+        rl_set_error("%s: x and w must be 16-byte aligned", who);
+        return -1;
+    }
+    return 0;
+}
+
+int validate(const rl_token_logprob_args_t *a, const char *who)
+{
+    if (!a || !a->logprob || !a->lse) {
+        rl_set_error("%s: NULL argument", who);
+        return -1;
+    }
+    return validate(who, a->x, a->w, a->targets, a->rows, a->vocab, a->hidden, a->x_stride, a->w_stride, a->scale);
+}
+
+int validate(const rl_token_logprob_grad_args_t *a, const char *who)
+{
+    if (!a || !a->lse || !a->grad_logprob || (!a->dx && !a->dw)) {
+        rl_set_error("%s: NULL argument", who);
+        return -1;
+    }
+    if (validate(who, a->x, a->w, a->targets, a->rows, a->vocab, a->hidden, a->x_stride, a->w_stride, a->scale))
+        return -1;
+    if ((a->dx && (a->dx_stride < a->hidden || a->dx_stride % 8 != 0)) ||
+        (a->dw && (a->dw_stride < a->hidden || a->dw_stride % 8 != 0))) {
+        rl_set_error("%s: strides dx %u dw %u (multiples of 8 from hidden on)", who, a->dx_stride, a->dw_stride);
+        return -1;
+    }
+    if (((uintptr_t)a->dx | (uintptr_t)a->dw) % 16 != 0) {
+        rl_set_error("%s: dx and dw must be 16-byte aligned", who);
+        return -1;
+    }
+    return 0;
+}
+
+int short_workspace(const char *who, const void *ws, size_t bytes, size_t need)
+{
+    if (ws && bytes >= need && (uintptr_t)ws % 16 == 0)
+        return 0;
+    rl_set_error("%s: workspace %zu bytes < %zu required (16-byte aligned)", who, bytes, need);
+    return -1;
+}
+
+}  // namespace
+
+extern "C" size_t rl_hip_token_logprob_workspace(const rl_token_logprob_args_t *a)
+{
+    if (validate(a, "rl_hip_token_logprob_workspace") || rl_require_open("rl_hip_token_logprob_workspace"))
+        return 0;
+    // (the smallest tiles have a slot for 32 entries)
+    return up256((uint64_t)tiles_of(a->vocab, 64) * 2 * std::min(a->rows, 256u) * 8) +
+           up256((uint64_t)slots_of<RowsMany>(a->vocab) * a->rows * 8) + up256(a->rows * 4ull);
+}
+
+extern "C" int rl_hip_token_logprob(const rl_token_logprob_args_t *a)
+{
+    const char *who = "rl_hip_token_logprob";
+    if (validate(a, who) || rl_require_open(who))
+        return -1;
+    const uint32_t slots = slots_of(a->rows, a->vocab);
+    const size_t part = up256((uint64_t)slots * a->rows * 8);
+    if (short_workspace(who, a->workspace, a->workspace_bytes, part + up256(a->rows * 4ull)))
+        return -1;
+    LogitParams p = {};
+    p.w = GemmOperand{(const uint16_t *)a->w, a->w_stride, a->vocab, a->hidden};
+    p.x = GemmOperand{(const uint16_t *)a->x, a->x_stride, a->rows, a->hidden};
+    p.targets = a->targets;
+    p.scale = a->scale != 0.f ? a->scale : 1.f;
+    p.rows = a->rows;
+    p.vocab = a->vocab;
+    p.part = (rl_f32x2 *)a->workspace;
+    p.hit = (float *)((uint8_t *)a->workspace + part);
+    if (a->rows <= 32    ? launch_stats<Rows32, true>(p)
+        : a->rows <= 64  ? launch_stats<Rows64, true>(p)
+        : a->rows <= 128 ? launch_stats<Rows128, true>(p)
+        : a->rows <= 256 ? launch_stats<Rows256, false>(p)
+                         : launch_stats<RowsMany, false>(p))
+        return -1;
+    hipLaunchKernelGGL(token_logprob_kernel, dim3(tiles_of(a->rows, 16)), dim3(256), 0, rl_stream(), p.part, p.hit,
+                       a->targets, a->rows, a->vocab, slots, a->logprob, a->lse);
+    return rl_check_launch("token_logprob_kernel launch");
+}
+
+extern "C" size_t rl_hip_token_logprob_grad_workspace(const rl_token_logprob_grad_args_t *a)
+{
+    if (validate(a, "rl_hip_token_logprob_grad_workspace") || rl_require_open("rl_hip_token_logprob_grad_workspace"))
+        return 0;
+    return plan_of(a->rows, a->vocab, a->hidden).most;
+}
+
+extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
+{
+    const char *who = "rl_hip_token_logprob_grad";
+    if (validate(a, who) || rl_require_open(who))
+        return -1;
+    const GradPlan pl = plan_of(a->rows, a->vocab, a->hidden);
+    if (short_workspace(who, a->workspace, a->workspace_bytes, pl.d + pl.x + pl.part))
+        return -1;
+    uint16_t *d = (uint16_t *)a->workspace, *x = (uint16_t *)((uint8_t *)d + pl.d);
+    float *part = (float *)((uint8_t *)x + pl.x);
+    if (a->dw) {
+        hipLaunchKernelGGL(token_rows_kernel, dim3(std::min(pl.rows_pad, 65535u)), dim3(256), 0, rl_stream(),
+                           (const uint16_t *)a->x, a->x_stride, a->targets, a->rows, pl.rows_pad, a->vocab, a->hidden, x);
+        if (rl_check_launch("token_rows_kernel launch"))
+            return -1;
+    }
+    LogitParams p = {};
+    p.x = GemmOperand{(const uint16_t *)a->x, a->x_stride, a->rows, a->hidden};
+    p.targets = a->targets;
+    p.scale = a->scale != 0.f ? a->scale : 1.f;
+    p.rows = a->rows;
+    p.vocab = a->vocab;
+    p.lse = a->lse;
+    p.grad = a->grad_logprob;
+    p.d = d;
+    p.rows_pad = pl.rows_pad;
+    p.pitch = pl.width;
+    DxParams dx = {};
+    dx.targets = a->targets;
+    dx.rows = a->rows;
+    dx.vocab = a->vocab;
+    dx.hidden = a->hidden;
+    dx.part = pl.direct ? nullptr : part;
+    dx.dx = (uint16_t *)a->dx;
+    dx.dx_ld = a->dx_stride;
+    for (uint32_t v0 = 0; v0 < a->vocab; v0 += pl.width) {
+        const uint32_t n = std::min(pl.width, a->vocab - v0);
+        const uint16_t *w = (const uint16_t *)a->w + (uint64_t)v0 * a->w_stride;
+        p.w = GemmOperand{w, a->w_stride, n, a->hidden};
+        p.v0 = v0;
+        if (a->rows <= 32    ? launch_delta<Rows32, true>(p)
+            : a->rows <= 64  ? launch_delta<Rows64, true>(p)
+            : a->rows <= 128 ? launch_delta<Rows128, true>(p)
+            : a->rows <= 256 ? launch_delta<Rows256, false>(p)
+                             : launch_delta<RowsMany, false>(p))
+            return -1;
+        if (a->dx) {
+            dx.w = GemmOperand{w, a->w_stride, a->hidden, n};
+            dx.d = GemmOperand{d, pl.width, pl.rows_pad, n};
+            dx.steps = tiles_of(n, kGemmK);
+            dx.split = pl.split;
+            dx.add = v0 != 0;
+            if (a->rows <= 32    ? launch_dx<Dx32>(dx)
+                : a->rows <= 64  ? launch_dx<Dx64>(dx)
+                : a->rows <= 128 ? launch_dx<Dx128>(dx)
+                                 : launch_dx<DxMany>(dx))
+                return -1;
+        }
+        if (a->dw) {
+            DwParams dw;
+            dw.x = GemmOperand{x, a->hidden, a->hidden, pl.rows_pad};
+            dw.d = GemmOperand{d, pl.width, pl.width, pl.rows_pad};
+            dw.entries = n;
+            dw.hidden = a->hidden;
+            dw.m_tiles = tiles_of(n, Dw::BM);
+            dw.n_tiles = tiles_of(a->hidden, Dw::BN);
+            dw.steps = pl.rows_pad / kGemmK;
+            dw.dw = (uint16_t *)a->dw + (uint64_t)v0 * a->dw_stride;
+            dw.dw_ld = a->dw_stride;
+            hipLaunchKernelGGL(token_dw_kernel<Dw>, dim3(grid_of(dw.m_tiles * dw.n_tiles)), dim3(Dw::WAVES * 64), 0,
+                               rl_stream(), dw);
+            if (rl_check_launch("token_dw_kernel launch"))
+                return -1;
+        }
+    }
+    if (a->dx && !pl.direct) {
+        hipLaunchKernelGGL(token_dx_sum_kernel, dim3(std::min(a->rows, 65535u)), dim3(256), 0, rl_stream(), dx);
+        if (rl_check_launch("token_dx_sum_kernel launch"))
+            return -1;
+    }
+    return 0;
+}

@@ -279,6 +279,21 @@ class ProjArgs(C.Structure):
                 ("w_stride", C.c_uint32), ("logits_stride", C.c_uint32)]
 
 
+class TokenLogprobArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("targets", C.c_void_p), ("rows", C.c_uint32),
+                ("vocab", C.c_uint32), ("hidden", C.c_uint32), ("x_stride", C.c_uint32), ("w_stride", C.c_uint32),
+                ("scale", C.c_float), ("logprob", C.c_void_p), ("lse", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
+class TokenLogprobGradArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("targets", C.c_void_p), ("rows", C.c_uint32),
+                ("vocab", C.c_uint32), ("hidden", C.c_uint32), ("x_stride", C.c_uint32), ("w_stride", C.c_uint32),
+                ("scale", C.c_float), ("lse", C.c_void_p), ("grad_logprob", C.c_void_p), ("dx", C.c_void_p),
+                ("dw", C.c_void_p), ("dx_stride", C.c_uint32), ("dw_stride", C.c_uint32), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
 class RewardArgs(C.Structure):
     _fields_ = [("tokens", C.c_void_p), ("n_tokens", C.c_void_p), ("targets", C.c_void_p),
                 ("rollouts", C.c_uint32), ("group_size", C.c_uint32), ("token_stride", C.c_uint32),
@@ -392,6 +407,10 @@ def load(path: str = LIB_PATH) -> C.CDLL:
         "rl_hip_rope_append": (i32, [C.POINTER(RopeAppendArgs)]),
         "rl_hip_attn_chunk_workspace": (sz, [C.POINTER(AttnChunkArgs)]),
         "rl_hip_attn_chunk": (i32, [C.POINTER(AttnChunkArgs)]),
+        "rl_hip_token_logprob_workspace": (sz, [C.POINTER(TokenLogprobArgs)]),
+        "rl_hip_token_logprob": (i32, [C.POINTER(TokenLogprobArgs)]),
+        "rl_hip_token_logprob_grad_workspace": (sz, [C.POINTER(TokenLogprobGradArgs)]),
+        "rl_hip_token_logprob_grad": (i32, [C.POINTER(TokenLogprobGradArgs)]),
         "rl_rope_freqs": (i32, [vp, u32, C.c_double]),
         "rl_hip_logits_proj": (i32, [C.POINTER(ProjArgs)]),
         "rl_hip_reward_advantage": (i32, [C.POINTER(RewardArgs)]),
@@ -766,6 +785,42 @@ def attn_chunk_workspace(args: AttnChunkArgs) -> DeviceBuffer:
 def attn_chunk(args: AttnChunkArgs) -> None:
     """Causal attention of each row's newest tokens over the 16-bit arena."""
     check(lib().rl_hip_attn_chunk(C.byref(args)), "rl_hip_attn_chunk")
+
+
+def token_logprob_workspace_bytes(args: TokenLogprobArgs) -> int:
+    n = lib().rl_hip_token_logprob_workspace(C.byref(args))
+    if n == 0:
+        raise RlrtError(f"rl_hip_token_logprob_workspace: {_err()}")
+    return int(n)
+
+
+def token_logprob_workspace(args: TokenLogprobArgs) -> DeviceBuffer:
+    ws = DeviceBuffer(token_logprob_workspace_bytes(args))
+    args.workspace, args.workspace_bytes = ws.ptr, ws.nbytes
+    return ws
+
+
+def token_logprob(args: TokenLogprobArgs) -> None:
+    """Log probabilities of given tokens under a vocabulary projection."""
+    check(lib().rl_hip_token_logprob(C.byref(args)), "rl_hip_token_logprob")
+
+
+def token_logprob_grad_workspace_bytes(args: TokenLogprobGradArgs) -> int:
+    n = lib().rl_hip_token_logprob_grad_workspace(C.byref(args))
+    if n == 0:
+        raise RlrtError(f"rl_hip_token_logprob_grad_workspace: {_err()}")
+    return int(n)
+
+
+def token_logprob_grad_workspace(args: TokenLogprobGradArgs) -> DeviceBuffer:
+    ws = DeviceBuffer(token_logprob_grad_workspace_bytes(args))
+    args.workspace, args.workspace_bytes = ws.ptr, ws.nbytes
+    return ws
+
+
+def token_logprob_grad(args: TokenLogprobGradArgs) -> None:
+    """The gradients of the hidden states and the projection by the log probabilities'."""
+    check(lib().rl_hip_token_logprob_grad(C.byref(args)), "rl_hip_token_logprob_grad")
 
 
 def kv8_append(args: Kv8AppendArgs) -> None:

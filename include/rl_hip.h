@@ -356,6 +356,66 @@ typedef struct {
 
 int rl_hip_logits_proj(const rl_logits_proj_args_t *args);
 
+/* ---- log probabilities of given tokens, and their gradients ----------------------
+ * No reference function. What a policy's training step needs beside the
+ * advantages: with the logits z[r][v] = scale * (x_r . w_v) of the projection
+ * above (bf16 operands, fp32 sums; scale is 1 / temperature),
+ *   lse[r] = log sum_v exp z[r][v]    logprob[r] = z[r][targets[r]] - lse[r]
+ * without keeping the logits. A row whose target is `vocab` or more (the places
+ * behind a rollout's end, say) has logprob 0, its lse all the same.
+ *
+ * rl_hip_token_logprob_grad is its gradient: from lse and grad_logprob[r], the
+ * derivative of the loss by logprob[r] (for -mean(advantage * logprob): the
+ * negative advantage over the number of tokens),
+ *   D[r][v] = scale * grad_logprob[r] * (1[v = targets[r]] - exp(z[r][v] - lse[r]))
+ *   dx = D w    dw = D^T x
+ * in pieces of the vocabulary whose logits are computed again; D is rounded to
+ * bf16, sums are fp32 and each result is rounded once. dx or dw may be NULL.
+ * Rows without a target have no part in either, whatever they hold, and get
+ * zeros in dx. The same call gives the same bits. */
+typedef struct {
+    const void *x;               /* device [rows][x_stride] bf16, 16-byte aligned */
+    const void *w;               /* device [vocab][w_stride] bf16, 16-byte aligned */
+    const uint32_t *targets;     /* device [rows] */
+    uint32_t rows;               /* 1 .. 2^20; below 2^23 blocks of 256 rows x 256 entries */
+    uint32_t vocab;              /* 1 .. 2^24 */
+    uint32_t hidden;             /* a multiple of 64 up to 2^16 */
+    uint32_t x_stride;           /* elements: multiples of 8 from hidden to 2^22 */
+    uint32_t w_stride;
+    float scale;                 /* positive; 0 selects 1 */
+    float *logprob;              /* device [rows] */
+    float *lse;                  /* device [rows] */
+    void *workspace;             /* device, >= rl_hip_token_logprob_workspace() */
+    size_t workspace_bytes;
+} rl_token_logprob_args_t;
+
+/* Both queries: enough also for every call with at most these rows, vocab and hidden. */
+size_t rl_hip_token_logprob_workspace(const rl_token_logprob_args_t *args);
+int rl_hip_token_logprob(const rl_token_logprob_args_t *args);
+
+typedef struct {
+    const void *x;               /* x to scale: as above */
+    const void *w;
+    const uint32_t *targets;
+    uint32_t rows;
+    uint32_t vocab;
+    uint32_t hidden;
+    uint32_t x_stride;
+    uint32_t w_stride;
+    float scale;
+    const float *lse;            /* device [rows], from rl_hip_token_logprob */
+    const float *grad_logprob;   /* device [rows] */
+    void *dx;                    /* device [rows][dx_stride] bf16, 16-byte aligned, or NULL */
+    void *dw;                    /* device [vocab][dw_stride] bf16, 16-byte aligned, or NULL */
+    uint32_t dx_stride;          /* elements: multiples of 8 from hidden on */
+    uint32_t dw_stride;
+    void *workspace;             /* device, >= rl_hip_token_logprob_grad_workspace() */
+    size_t workspace_bytes;
+} rl_token_logprob_grad_args_t;
+
+size_t rl_hip_token_logprob_grad_workspace(const rl_token_logprob_grad_args_t *args);
+int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *args);
+
 /* ---- reward and group advantage ---------------------------------------------
  * Replaces reward_score_kernel (cu/reward.cu:4-15) and adds the GRPO group
  * advantage (no reference function). Rollout r belongs to group
