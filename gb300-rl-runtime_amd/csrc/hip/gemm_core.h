@@ -228,46 +228,55 @@ struct Gemm {
         rl_wait_lgkmcnt0();  // (the reads behind the last step)
     }
 
-    // f(m, n, x): four results of row m, columns n .. n + 3, at a time; m, n relative to the tile.
-    template <typename F>
-    static __device__ __forceinline__ void each4(const Acc &acc, F f)
+    // Hands the results out in 16-byte pieces of rows, f(m, n, w): row m and column n of the tile on, as bf16 (eight
+    // columns) or as floats (four), so that a wave's pieces lie 64 * TN (floats: 128 * TN) bytes one behind the other in
+    // each row. They change lanes in LDS, which must be free of operands: 32 rows of a wave at a time.
+    template <bool FLOATS, typename F>
+    static __device__ __forceinline__ void each(const Acc &acc, uint8_t *smem_, F f)
     {
+        constexpr uint32_t NC = TN * (FLOATS ? 8 : 4), OUT = 32 * NC / 64;  // 16-byte chunks of a row; pieces per lane
+        static_assert(WAVES * 32 * NC * 16 <= LDS, "room for the waves' rows");
         const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const uint32_t wn = wave % WN, wm = wave / WN, hf = lane >> 5;
+        const uint32_t wn = wave % WN, wm = wave / WN, hf = lane >> 5, r = lane & 31u;
+        RL_LDS uint8_t *own = (RL_LDS uint8_t *)smem_ + wave * (32 * NC * 16);
+        // (16 neighbouring lanes write the same chunk of 16 rows, and read chunks that follow each other: both meet
+        // every bank once)
+        auto place = [&](uint32_t row, uint32_t c) {
+            const uint32_t swz = NC >= 16 ? row & 15u : NC == 8 ? (row >> 1) & 7u : (row >> 2) & 3u;
+            return (RL_LDS rl_u32x4 *)(own + row * (NC * 16) + ((c ^ swz) << 4));
+        };
 #pragma unroll
-        for (int b = 0; b < TM; b++)
+        for (int b = 0; b < TM; b++) {
 #pragma unroll
             for (int a = 0; a < TN; a++)
 #pragma unroll
-                for (int c = 0; c < 4; c++)
-                    f((wm * TM + b) * 32 + (lane & 31u), (wn * TN + a) * 32 + 8 * c + 4 * hf,
-                      rl_f32x4{acc[a][b][4 * c], acc[a][b][4 * c + 1], acc[a][b][4 * c + 2], acc[a][b][4 * c + 3]});
-    }
-
-    // f(m, n, w): eight results of row m, columns n .. n + 7, as bf16, at a time.
-    template <typename F>
-    static __device__ __forceinline__ void each8(const Acc &acc, F f)
-    {
-        const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const uint32_t wn = wave % WN, wm = wave / WN, hf = lane >> 5;
+                for (int c = 0; c < 4; c++) {
+                    if constexpr (FLOATS) {
+                        *place(r, 8 * a + 2 * c + hf) = rl_u32x4{
+                            __float_as_uint(acc[a][b][4 * c]), __float_as_uint(acc[a][b][4 * c + 1]),
+                            __float_as_uint(acc[a][b][4 * c + 2]), __float_as_uint(acc[a][b][4 * c + 3])};
+                    } else if (c % 2 == 0) {
+                        // lanes l and l + 32 hold four columns each of both eights: each takes a whole one
+                        rl_u32x4 w;
 #pragma unroll
-        for (int b = 0; b < TM; b++)
-#pragma unroll
-            for (int a = 0; a < TN; a++)
-#pragma unroll
-                for (int c = 0; c < 4; c += 2) {
-                    // lanes l and l + 32 hold four columns each of both eights: each takes a whole one
-                    rl_u32x4 w;
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const uint32_t x = pack(acc[a][b][4 * c + 2 * e], acc[a][b][4 * c + 2 * e + 1]);
-                        const uint32_t y = pack(acc[a][b][4 * c + 4 + 2 * e], acc[a][b][4 * c + 5 + 2 * e]);
-                        const auto h = __builtin_amdgcn_permlane32_swap(x, y, false, false);
-                        w[e] = h[0];
-                        w[2 + e] = h[1];
+                        for (int e = 0; e < 2; e++) {
+                            const uint32_t x = pack(acc[a][b][4 * c + 2 * e], acc[a][b][4 * c + 2 * e + 1]);
+                            const uint32_t y = pack(acc[a][b][4 * c + 4 + 2 * e], acc[a][b][4 * c + 5 + 2 * e]);
+                            const auto h = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+                            w[e] = h[0];
+                            w[2 + e] = h[1];
+                        }
+                        *place(r, 4 * a + c + hf) = w;
                     }
-                    f((wm * TM + b) * 32 + (lane & 31u), (wn * TN + a) * 32 + 8 * (c + hf), w);
                 }
+            rl_wave_lds_fence();
+#pragma unroll
+            for (uint32_t j = 0; j < OUT; j++) {
+                const uint32_t row = (j * 64 + lane) / NC, c = (j * 64 + lane) % NC;
+                f((wm * TM + b) * 32 + row, wn * TN * 32 + c * (FLOATS ? 4 : 8), *place(row, c));
+            }
+            rl_wave_lds_fence();
+        }
     }
 
     static __device__ __forceinline__ uint32_t pack(float x, float y)

@@ -22,6 +22,12 @@
 #include "rl_hip.h"
 #include "rl_hip_internal.h"
 
+#ifndef DWFEW
+#define DWFEW 512
+#endif
+#ifndef ROT256
+#define ROT256 true
+#endif
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -38,6 +44,15 @@ __device__ __forceinline__ float pair_sum(float x)
     return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
 
+// Maximum and sum of exponentials of two sets together.
+__device__ __forceinline__ rl_f32x2 join(rl_f32x2 x, rl_f32x2 y)
+{
+    // (a set without a maximum has the sum 0, or none that is a number)
+    const float top = fmaxf(x[0], y[0]);
+    return rl_f32x2{top, x[1] * (x[0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((x[0] - top) * kLog2e)) +
+                             y[1] * (y[0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((y[0] - top) * kLog2e))};
+}
+
 struct LogitParams {
     GemmOperand w, x;        // w: the piece's rows
     const uint32_t *targets;
@@ -45,7 +60,7 @@ struct LogitParams {
     uint32_t rows, vocab, v0;  // v0: the piece's first entry; vocab: of all
     uint32_t m_tiles, n_tiles;
     // statistics
-    rl_f32x2 *part;          // [n_tiles * WN][rows]: maximum and sum
+    rl_f32x2 *part;          // [n_tiles][rows]: maximum and sum
     float *hit;              // [rows]: the target's logit
     // gradient
     const float *lse, *grad;
@@ -80,9 +95,11 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_stats_kernel(LogitParams 
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hf = lane >> 5;
     const uint32_t wn = wave % G::WN, wm = wave / G::WN, n0 = nt * G::BN + wn * G::TN * 32;
     const bool whole = n0 + G::TN * 32 <= p.vocab;
+    rl_f32x2 *all = (rl_f32x2 *)smem;  // [WN][BM]
+    __syncthreads();                   // (nobody reads operands any more)
 #pragma unroll
     for (int b = 0; b < G::TM; b++) {
-        const uint32_t row = m0 + (wm * G::TM + b) * 32 + (lane & 31);
+        const uint32_t at_row = (wm * G::TM + b) * 32 + (lane & 31), row = m0 + at_row;
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int a = 0; a < G::TN; a++)
@@ -102,9 +119,9 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_stats_kernel(LogitParams 
             for (int r = 0; r < 16; r++)
                 sum += __builtin_amdgcn_exp2f((acc[a][b][r] - ref) * kLog2e);
         sum = pair_sum(sum);
+        if (hf == 0)
+            all[wn * G::BM + at_row] = rl_f32x2{top, sum};
         if (row < p.rows) {
-            if (hf == 0)
-                p.part[(uint64_t)(nt * G::WN + wn) * p.rows + row] = rl_f32x2{top, sum};
             const uint32_t t = p.targets[row], at = t - n0;
             if (t < p.vocab && at < G::TN * 32 && (at >> 2 & 1) == hf) {
 #pragma unroll
@@ -116,40 +133,49 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_stats_kernel(LogitParams 
             }
         }
     }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < G::BM && m0 + i < p.rows; i += G::WAVES * 64) {
+        rl_f32x2 x = all[i];
+#pragma unroll
+        for (int w = 1; w < G::WN; w++)
+            x = join(x, all[w * G::BM + i]);
+        p.part[(uint64_t)nt * p.rows + m0 + i] = x;
+    }
 }
 
-// Joins the statistics of 16 rows: 16 threads a row, four shares at a time each.
+// Joins the tiles' statistics of R rows per workgroup: 256 / R threads a row, each with eight tiles' at a time.
+template <int R>
 __global__ __launch_bounds__(256) void token_logprob_kernel(const rl_f32x2 *part, const float *hit,
                                                             const uint32_t *targets, uint32_t rows, uint32_t vocab,
                                                             uint32_t slots, float *logprob, float *lse)
 {
-    __shared__ rl_f32x2 all[16][16];
-    const uint32_t r = threadIdx.x % 16, y = threadIdx.x / 16, row = blockIdx.x * 16 + r, at = min(row, rows - 1);
-    float top = -INFINITY, sum = 0.f;
-    auto join = [&](float m, float l) {
-        // (before a maximum, a sum is 0 or no number)
-        const float t = fmaxf(top, m);
-        sum = sum * (top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top - t) * kLog2e)) +
-              l * (m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - t) * kLog2e));
-        top = t;
-    };
-    for (uint32_t s = y; s < slots; s += 64) {
-        rl_f32x2 x[4];
+    constexpr uint32_t PER = 256 / R;
+    __shared__ rl_f32x2 all[4][R];
+    const uint32_t r = threadIdx.x % R, y = threadIdx.x / R, row = blockIdx.x * R + r, at = min(row, rows - 1);
+    rl_f32x2 x = {-INFINITY, 0.f};
+    for (uint32_t s = y; s < slots; s += 8 * PER) {
+        rl_f32x2 in[8];
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++)
-            x[i] = part[(uint64_t)min(s + 16 * i, slots - 1) * rows + at];
+        for (uint32_t i = 0; i < 8; i++)
+            in[i] = part[(uint64_t)min(s + PER * i, slots - 1) * rows + at];
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++)
-            if (s + 16 * i < slots)
-                join(x[i][0], x[i][1]);
+        for (uint32_t i = 0; i < 8; i++)
+            if (s + PER * i < slots)
+                x = join(x, in[i]);
     }
-    all[y][r] = rl_f32x2{top, sum};
+#pragma unroll
+    for (int d = R; d < 64; d *= 2)
+        x = join(x, rl_f32x2{__shfl_xor(x[0], d), __shfl_xor(x[1], d)});
+    if ((threadIdx.x & 63) < R)
+        all[threadIdx.x >> 6][r] = x;
     __syncthreads();
-    if (y != 0 || row >= rows)
+    if (threadIdx.x >= R || row >= rows)
         return;
-    for (uint32_t i = 1; i < 16; i++)
-        join(all[i][r][0], all[i][r][1]);
-    const float z = top == -INFINITY && sum == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + logf(sum);
+#pragma unroll
+    for (int i = 1; i < 4; i++)
+        x = join(x, all[i][r]);
+    // (all of them -infinity: so is the logarithm)
+    const float z = x[0] == -INFINITY ? (x[1] == 0.f ? -INFINITY : x[1]) : x[0] + logf(x[1]);
     lse[row] = z;
     logprob[row] = targets[row] < vocab ? hit[row] - z : 0.f;
 }
@@ -183,7 +209,8 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_delta_kernel(LogitParams 
             }
     }
     uint16_t *d = p.d + nt * G::BN;
-    G::each8(acc, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
+    __syncthreads();  // (nobody reads operands any more)
+    G::template each<false>(acc, smem, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
         if (m0 + m < p.rows_pad)
             *(rl_u32x4 *)(d + (uint64_t)(m0 + m) * p.pitch + n) = w;
         if (G::BM == 32)  // (rows_pad is 64)
@@ -228,9 +255,11 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_dx_kernel(DxParams p)
     const uint32_t k1 = (uint32_t)((uint64_t)(share + 1) * p.steps / p.split);
     typename G::Acc acc;
     G::run(p.w, p.d, n0, m0, k0, k1, 0, smem, acc);
+    __syncthreads();  // (nobody reads operands any more)
     if (p.part) {
         float *part = p.part + (uint64_t)share * p.rows * p.hidden;
-        G::each4(acc, [&](uint32_t m, uint32_t n, rl_f32x4 x) {
+        G::template each<true>(acc, smem, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
+            rl_f32x4 x = __builtin_bit_cast(rl_f32x4, w);
             if (m0 + m < p.rows && n0 + n < p.hidden) {
                 float *at = part + (uint64_t)(m0 + m) * p.hidden + n0 + n;
                 if (p.add) {
@@ -244,7 +273,7 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_dx_kernel(DxParams p)
         });
         return;
     }
-    G::each8(acc, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
+    G::template each<false>(acc, smem, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
         if (m0 + m < p.rows && n0 + n < p.hidden) {
             if (p.targets[m0 + m] >= p.vocab)
                 w = rl_u32x4{0, 0, 0, 0};
@@ -260,11 +289,17 @@ __global__ __launch_bounds__(256) void token_dx_sum_kernel(DxParams p)
         for (uint32_t c = threadIdx.x; c < p.hidden / 4; c += 256) {
             rl_f32x4 x = {0.f, 0.f, 0.f, 0.f};
             const float *at = p.part + (uint64_t)row * p.hidden + c * 4;
-            for (uint32_t s = 0; s < p.split; s++) {
-                const rl_f32x4 y = *(const rl_f32x4 *)(at + (uint64_t)s * p.rows * p.hidden);
+            for (uint32_t s = 0; s < p.split; s += 8) {
+                rl_f32x4 y[8];
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    x[e] += y[e];
+                for (uint32_t i = 0; i < 8; i++)
+                    y[i] = *(const rl_f32x4 *)(at + (uint64_t)min(s + i, p.split - 1) * p.rows * p.hidden);
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++)
+                    if (s + i < p.split)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            x[e] += y[i][e];
             }
             rl_u32x2 w = {(uint32_t)to16<0>(x[0]) | (uint32_t)to16<0>(x[1]) << 16,
                           (uint32_t)to16<0>(x[2]) | (uint32_t)to16<0>(x[3]) << 16};
@@ -292,7 +327,8 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_dw_kernel(DwParams p)
     const uint32_t m0 = mt * G::BM, n0 = nt * G::BN;
     typename G::Acc acc;
     G::run(p.x, p.d, n0, m0, 0, p.steps, 0, smem, acc);
-    G::each8(acc, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
+    __syncthreads();  // (nobody reads operands any more)
+    G::template each<false>(acc, smem, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
         if (m0 + m < p.entries && n0 + n < p.hidden)
             *(rl_u32x4 *)(p.dw + (m0 + m) * p.dw_ld + n0 + n) = w;
     });
@@ -309,15 +345,17 @@ using RowsMany = Gemm<4, 2, 2, 4, 2, false, false>;  // 256 x 256
 using Dx32 = Gemm<1, 4, 1, 1, 4, true, false>;       // 128 x 32
 using Dx64 = Gemm<1, 4, 2, 1, 3, true, false>;       // 128 x 64
 using Dx128 = Gemm<1, 4, 2, 2, 4, true, false>;      // 128 x 128
+using Dx256 = Gemm<2, 2, 2, 4, 3, true, false>;      // 128 x 256
 using DxMany = Gemm<4, 2, 2, 4, 2, true, false>;     // 256 x 256
 // (n along hidden, m along the vocabulary)
-using Dw = Gemm<4, 2, 2, 4, 2, true, true>;          // 256 x 256
+using DwFew = Gemm<2, 2, 1, 4, 2, true, true>;       // 128 x 128
+using DwMany = Gemm<4, 2, 2, 4, 2, true, true>;      // 256 x 256
 
 uint32_t tiles_of(uint64_t n, uint32_t per) { return (uint32_t)((n + per - 1) / per); }
 uint32_t grid_of(uint32_t tiles) { return (tiles + 7) / 8 * 8; }
 
 template <typename G>
-uint32_t slots_of(uint32_t vocab) { return tiles_of(vocab, G::BN) * G::WN; }
+uint32_t slots_of(uint32_t vocab) { return tiles_of(vocab, G::BN); }
 
 uint32_t slots_of(uint32_t rows, uint32_t vocab)
 {
@@ -358,6 +396,15 @@ int launch_dx(DxParams p)
     return rl_check_launch("token_dx_kernel launch");
 }
 
+template <typename G>
+int launch_dw(DwParams p)
+{
+    p.m_tiles = tiles_of(p.entries, G::BM);
+    p.n_tiles = tiles_of(p.hidden, G::BN);
+    hipLaunchKernelGGL(token_dw_kernel<G>, dim3(grid_of(p.m_tiles * p.n_tiles)), dim3(G::WAVES * 64), 0, rl_stream(), p);
+    return rl_check_launch("token_dw_kernel launch");
+}
+
 struct GradPlan {
     uint32_t rows_pad, width;  // rows of D, and its columns: entries of a piece, a multiple of 256
     uint32_t split;            // shares of a piece's vocabulary for dx
@@ -391,6 +438,8 @@ GradPlan plan_of(uint32_t rows, uint32_t vocab, uint32_t hidden)
         dx_shape<Dx64>(rows, hidden, 2, tiles, at_once);
     else if (rows <= 128)
         dx_shape<Dx128>(rows, hidden, 1, tiles, at_once);
+    else if (rows <= 256)
+        dx_shape<Dx256>(rows, hidden, 1, tiles, at_once);
     else
         dx_shape<DxMany>(rows, hidden, 1, tiles, at_once);
     // shares of eight steps at least, of the last piece too
@@ -485,8 +534,8 @@ extern "C" size_t rl_hip_token_logprob_workspace(const rl_token_logprob_args_t *
 {
     if (validate(a, "rl_hip_token_logprob_workspace") || rl_require_open("rl_hip_token_logprob_workspace"))
         return 0;
-    // (the smallest tiles have a slot for 32 entries)
-    return up256((uint64_t)tiles_of(a->vocab, 64) * 2 * std::min(a->rows, 256u) * 8) +
+    // (few rows have the smallest tiles)
+    return up256((uint64_t)slots_of<Rows32>(a->vocab) * std::min(a->rows, 256u) * 8) +
            up256((uint64_t)slots_of<RowsMany>(a->vocab) * a->rows * 8) + up256(a->rows * 4ull);
 }
 
@@ -511,11 +560,15 @@ extern "C" int rl_hip_token_logprob(const rl_token_logprob_args_t *a)
     if (a->rows <= 32    ? launch_stats<Rows32, true>(p)
         : a->rows <= 64  ? launch_stats<Rows64, true>(p)
         : a->rows <= 128 ? launch_stats<Rows128, true>(p)
-        : a->rows <= 256 ? launch_stats<Rows256, false>(p)
+        : a->rows <= 256 ? launch_stats<Rows256, ROT256>(p)
                          : launch_stats<RowsMany, false>(p))
         return -1;
-    hipLaunchKernelGGL(token_logprob_kernel, dim3(tiles_of(a->rows, 16)), dim3(256), 0, rl_stream(), p.part, p.hit,
-                       a->targets, a->rows, a->vocab, slots, a->logprob, a->lse);
+    if (slots > 128)
+        hipLaunchKernelGGL(token_logprob_kernel<4>, dim3(tiles_of(a->rows, 4)), dim3(256), 0, rl_stream(), p.part, p.hit,
+                           a->targets, a->rows, a->vocab, slots, a->logprob, a->lse);
+    else
+        hipLaunchKernelGGL(token_logprob_kernel<16>, dim3(tiles_of(a->rows, 16)), dim3(256), 0, rl_stream(), p.part,
+                           p.hit, a->targets, a->rows, a->vocab, slots, a->logprob, a->lse);
     return rl_check_launch("token_logprob_kernel launch");
 }
 
@@ -569,7 +622,7 @@ extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
         if (a->rows <= 32    ? launch_delta<Rows32, true>(p)
             : a->rows <= 64  ? launch_delta<Rows64, true>(p)
             : a->rows <= 128 ? launch_delta<Rows128, true>(p)
-            : a->rows <= 256 ? launch_delta<Rows256, false>(p)
+            : a->rows <= 256 ? launch_delta<Rows256, ROT256>(p)
                              : launch_delta<RowsMany, false>(p))
             return -1;
         if (a->dx) {
@@ -581,6 +634,7 @@ extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
             if (a->rows <= 32    ? launch_dx<Dx32>(dx)
                 : a->rows <= 64  ? launch_dx<Dx64>(dx)
                 : a->rows <= 128 ? launch_dx<Dx128>(dx)
+                : a->rows <= 256 ? launch_dx<Dx256>(dx)
                                  : launch_dx<DxMany>(dx))
                 return -1;
         }
@@ -590,14 +644,10 @@ extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
             dw.d = GemmOperand{d, pl.width, pl.width, pl.rows_pad};
             dw.entries = n;
             dw.hidden = a->hidden;
-            dw.m_tiles = tiles_of(n, Dw::BM);
-            dw.n_tiles = tiles_of(a->hidden, Dw::BN);
             dw.steps = pl.rows_pad / kGemmK;
             dw.dw = (uint16_t *)a->dw + (uint64_t)v0 * a->dw_stride;
             dw.dw_ld = a->dw_stride;
-            hipLaunchKernelGGL(token_dw_kernel<Dw>, dim3(grid_of(dw.m_tiles * dw.n_tiles)), dim3(Dw::WAVES * 64), 0,
-                               rl_stream(), dw);
-            if (rl_check_launch("token_dw_kernel launch"))
+            if (a->rows <= DWFEW ? launch_dw<DwFew>(dw) : launch_dw<DwMany>(dw))
                 return -1;
         }
     }
