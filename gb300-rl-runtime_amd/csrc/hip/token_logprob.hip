@@ -22,12 +22,6 @@
 #include "rl_hip.h"
 #include "rl_hip_internal.h"
 
-#ifndef DWFEW
-#define DWFEW 512
-#endif
-#ifndef ROT256
-#define ROT256 true
-#endif
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -330,7 +324,7 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_dw_kernel(DwParams p)
     __syncthreads();  // (nobody reads operands any more)
     G::template each<false>(acc, smem, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
         if (m0 + m < p.entries && n0 + n < p.hidden)
-            *(rl_u32x4 *)(p.dw + (m0 + m) * p.dw_ld + n0 + n) = w;
+            __builtin_nontemporal_store(w, (rl_u32x4 *)(p.dw + (m0 + m) * p.dw_ld + n0 + n));
     });
 }
 
@@ -348,8 +342,7 @@ using Dx128 = Gemm<1, 4, 2, 2, 4, true, false>;      // 128 x 128
 using Dx256 = Gemm<2, 2, 2, 4, 3, true, false>;      // 128 x 256
 using DxMany = Gemm<4, 2, 2, 4, 2, true, false>;     // 256 x 256
 // (n along hidden, m along the vocabulary)
-using DwFew = Gemm<2, 2, 1, 4, 2, true, true>;       // 128 x 128
-using DwMany = Gemm<4, 2, 2, 4, 2, true, true>;      // 256 x 256
+using Dw = Gemm<4, 2, 2, 4, 2, true, true>;          // 256 x 256
 
 uint32_t tiles_of(uint64_t n, uint32_t per) { return (uint32_t)((n + per - 1) / per); }
 uint32_t grid_of(uint32_t tiles) { return (tiles + 7) / 8 * 8; }
@@ -560,7 +553,7 @@ extern "C" int rl_hip_token_logprob(const rl_token_logprob_args_t *a)
     if (a->rows <= 32    ? launch_stats<Rows32, true>(p)
         : a->rows <= 64  ? launch_stats<Rows64, true>(p)
         : a->rows <= 128 ? launch_stats<Rows128, true>(p)
-        : a->rows <= 256 ? launch_stats<Rows256, ROT256>(p)
+        : a->rows <= 256 ? launch_stats<Rows256, true>(p)
                          : launch_stats<RowsMany, false>(p))
         return -1;
     if (slots > 128)
@@ -622,7 +615,7 @@ extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
         if (a->rows <= 32    ? launch_delta<Rows32, true>(p)
             : a->rows <= 64  ? launch_delta<Rows64, true>(p)
             : a->rows <= 128 ? launch_delta<Rows128, true>(p)
-            : a->rows <= 256 ? launch_delta<Rows256, ROT256>(p)
+            : a->rows <= 256 ? launch_delta<Rows256, true>(p)
                              : launch_delta<RowsMany, false>(p))
             return -1;
         if (a->dx) {
@@ -647,7 +640,7 @@ extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
             dw.steps = pl.rows_pad / kGemmK;
             dw.dw = (uint16_t *)a->dw + (uint64_t)v0 * a->dw_stride;
             dw.dw_ld = a->dw_stride;
-            if (a->rows <= DWFEW ? launch_dw<DwFew>(dw) : launch_dw<DwMany>(dw))
+            if (launch_dw<Dw>(dw))
                 return -1;
         }
     }
