@@ -301,6 +301,10 @@ int validate(const rl_rope_append_args_t *a)
             return -1;
         }
     }
+    if (a->q && a->q == a->q_out && (a->q_stride ? a->q_stride : qrow) != (a->q_out_stride ? a->q_out_stride : qrow)) {
+        rl_set_error("%s: q_out is q with another stride (%u and %u)", who, a->q_stride, a->q_out_stride);
+        return -1;
+    }
     if (((uintptr_t)a->arena_base | (uintptr_t)a->q | (uintptr_t)a->q_out | (uintptr_t)a->k_new | (uintptr_t)a->v_new |
          (uintptr_t)a->k_out) % 16 != 0 || (uintptr_t)a->freqs % 8 != 0) {
         rl_set_error("%s: arena_base and rows must be 16-byte aligned, freqs 8-byte aligned", who);

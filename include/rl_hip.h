@@ -372,7 +372,7 @@ int rl_hip_logits_proj(const rl_logits_proj_args_t *args);
  * in pieces of the vocabulary whose logits are computed again; D is rounded to
  * bf16, sums are fp32 and each result is rounded once. dx or dw may be NULL.
  * Rows without a target have no part in either, whatever they hold, and get
- * zeros in dx. The same call gives the same bits. */
+ * zeros in dx. Outputs may not overlap inputs. The same call gives the same bits. */
 typedef struct {
     const void *x;               /* device [rows][x_stride] bf16, 16-byte aligned */
     const void *w;               /* device [vocab][w_stride] bf16, 16-byte aligned */
