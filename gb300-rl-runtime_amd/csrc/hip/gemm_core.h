@@ -288,19 +288,23 @@ struct Gemm {
     }
 };
 
-// Workgroup b runs on XCD b % 8, each with its own L2. Each XCD gets a run of
-// tiles that follow each other in columns of up to 8 tiles along m, so that the 32
-// that it has at a time are about 8 x 4 and share their operands.
-__device__ __forceinline__ bool gemm_tile_of(uint32_t b, uint32_t m_tiles, uint32_t n_tiles, uint32_t &mt, uint32_t &nt)
+// Workgroup b runs on XCD b % 8, each with its own L2. Each XCD gets a run of `all` pieces of work that follow each
+// other (false: none is left).
+__device__ __forceinline__ bool gemm_run_of(uint32_t b, uint32_t all, uint32_t &t)
 {
-    const uint32_t all = m_tiles * n_tiles, per = (all + 7) / 8, t = b % 8 * per + b / 8;
-    if (b / 8 >= per || t >= all)
-        return false;
+    const uint32_t per = (all + 7) / 8;
+    t = b % 8 * per + b / 8;
+    return b / 8 < per && t < all;
+}
+
+// The tiles in columns of up to 8 along m, so that the 32 that an XCD has at a time are about 8 x 4 and share their
+// operands.
+__device__ __forceinline__ void gemm_tile_of(uint32_t t, uint32_t m_tiles, uint32_t n_tiles, uint32_t &mt, uint32_t &nt)
+{
     const uint32_t group = t / (8 * n_tiles), first = group * 8, high = min(8u, m_tiles - first);
     const uint32_t r = t - group * 8 * n_tiles;
     mt = first + r % high;
     nt = r / high;
-    return true;
 }
 
 }  // namespace

@@ -67,9 +67,10 @@ template <typename G, bool ROT>
 __device__ __forceinline__ bool logits_of(const LogitParams &p, uint8_t *smem, typename G::Acc &acc, uint32_t &m0,
                                           uint32_t &nt)
 {
-    uint32_t mt;
-    if (!gemm_tile_of(blockIdx.x, p.m_tiles, p.n_tiles, mt, nt))
+    uint32_t t, mt;
+    if (!gemm_run_of(blockIdx.x, p.m_tiles * p.n_tiles, t))
         return false;
+    gemm_tile_of(t, p.m_tiles, p.n_tiles, mt, nt);
     m0 = mt * G::BM;
     const uint32_t steps = p.x.k / kGemmK;
     // Each workgroup starts at another k: all starting at 0, they would read the same columns of rows that lie a
@@ -207,8 +208,8 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_delta_kernel(LogitParams 
     G::template each<false>(acc, smem, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
         if (m0 + m < p.rows_pad)
             *(rl_u32x4 *)(d + (uint64_t)(m0 + m) * p.pitch + n) = w;
-        if (G::BM == 32)  // (rows_pad is 64)
-            *(rl_u32x4 *)(d + (uint64_t)(m + 32) * p.pitch + n) = rl_u32x4{0, 0, 0, 0};
+        if (G::BM == 32 && m0 + 32 >= p.rows && m0 + 32 < p.rows_pad)  // (rows_pad is a multiple of 64)
+            *(rl_u32x4 *)(d + (uint64_t)(m0 + m + 32) * p.pitch + n) = rl_u32x4{0, 0, 0, 0};
     });
 }
 
@@ -241,10 +242,13 @@ template <typename G>
 __global__ __launch_bounds__(G::WAVES * 64) void token_dx_kernel(DxParams p)
 {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[G::LDS];
-    uint32_t mt, nt;
-    if (!gemm_tile_of(blockIdx.x, p.m_tiles, p.n_tiles, mt, nt))
+    // (an XCD's workgroups have the same share of the vocabulary, or two)
+    uint32_t t, mt, nt;
+    if (!gemm_run_of(blockIdx.x, p.m_tiles * p.n_tiles * p.split, t))
         return;
-    const uint32_t m0 = mt * G::BM, n0 = nt * G::BN, share = blockIdx.y;
+    const uint32_t share = t / (p.m_tiles * p.n_tiles);
+    gemm_tile_of(t - share * (p.m_tiles * p.n_tiles), p.m_tiles, p.n_tiles, mt, nt);
+    const uint32_t m0 = mt * G::BM, n0 = nt * G::BN;
     const uint32_t k0 = (uint32_t)((uint64_t)share * p.steps / p.split);
     const uint32_t k1 = (uint32_t)((uint64_t)(share + 1) * p.steps / p.split);
     typename G::Acc acc;
@@ -276,31 +280,34 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_dx_kernel(DxParams p)
     });
 }
 
-// dx from its shares, a workgroup a row at a time.
+// dx from its shares: 1,024 elements of a row per workgroup, in turn.
 __global__ __launch_bounds__(256) void token_dx_sum_kernel(DxParams p)
 {
-    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x)
-        for (uint32_t c = threadIdx.x; c < p.hidden / 4; c += 256) {
-            rl_f32x4 x = {0.f, 0.f, 0.f, 0.f};
-            const float *at = p.part + (uint64_t)row * p.hidden + c * 4;
-            for (uint32_t s = 0; s < p.split; s += 8) {
-                rl_f32x4 y[8];
+    const uint32_t across = (p.hidden + 1023) / 1024;
+    for (uint32_t i = blockIdx.x; i < p.rows * across; i += gridDim.x) {
+        const uint32_t row = i / across, c = (i - row * across) * 1024 + threadIdx.x * 4;
+        if (c >= p.hidden)
+            continue;
+        rl_f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        const float *at = p.part + (uint64_t)row * p.hidden + c;
+        for (uint32_t s = 0; s < p.split; s += 8) {
+            rl_f32x4 y[8];
 #pragma unroll
-                for (uint32_t i = 0; i < 8; i++)
-                    y[i] = *(const rl_f32x4 *)(at + (uint64_t)min(s + i, p.split - 1) * p.rows * p.hidden);
+            for (uint32_t k = 0; k < 8; k++)
+                y[k] = *(const rl_f32x4 *)(at + (uint64_t)min(s + k, p.split - 1) * p.rows * p.hidden);
 #pragma unroll
-                for (uint32_t i = 0; i < 8; i++)
-                    if (s + i < p.split)
+            for (uint32_t k = 0; k < 8; k++)
+                if (s + k < p.split)
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            x[e] += y[i][e];
-            }
-            rl_u32x2 w = {(uint32_t)to16<0>(x[0]) | (uint32_t)to16<0>(x[1]) << 16,
-                          (uint32_t)to16<0>(x[2]) | (uint32_t)to16<0>(x[3]) << 16};
-            if (p.targets[row] >= p.vocab)
-                w = rl_u32x2{0, 0};
-            *(rl_u32x2 *)(p.dx + row * p.dx_ld + c * 4) = w;
+                    for (int e = 0; e < 4; e++)
+                        x[e] += y[k][e];
         }
+        rl_u32x2 w = {(uint32_t)to16<0>(x[0]) | (uint32_t)to16<0>(x[1]) << 16,
+                      (uint32_t)to16<0>(x[2]) | (uint32_t)to16<0>(x[3]) << 16};
+        if (p.targets[row] >= p.vocab)
+            w = rl_u32x2{0, 0};
+        *(rl_u32x2 *)(p.dx + row * p.dx_ld + c) = w;
+    }
 }
 
 struct DwParams {
@@ -324,9 +331,10 @@ template <typename G>
 __global__ __launch_bounds__(G::WAVES * 64) void token_dw_kernel(DwParams p)
 {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[G::LDS];
-    uint32_t mt, nt;
-    if (!gemm_tile_of(blockIdx.x, p.m_tiles, p.n_tiles, mt, nt))
+    uint32_t t, mt, nt;
+    if (!gemm_run_of(blockIdx.x, p.m_tiles * p.n_tiles, t))
         return;
+    gemm_tile_of(t, p.m_tiles, p.n_tiles, mt, nt);
     const uint32_t m0 = mt * G::BM, n0 = nt * G::BN;
     typename G::Acc acc;
     G::run(p.x, p.d, n0, m0, 0, p.steps, 0, smem, acc);
@@ -338,12 +346,13 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_dw_kernel(DwParams p)
 }
 
 // ---- the host's side ----------------------------------------------------------------
-// Tiles by the number of rows (n along the vocabulary x m along the rows).
-using Rows32 = Gemm<1, 2, 1, 1, 4, false, false>;    // 64 x 32
-using Rows64 = Gemm<1, 2, 2, 1, 4, false, false>;    // 64 x 64
-using Rows128 = Gemm<1, 4, 2, 2, 4, false, false>;   // 128 x 128
-using Rows256 = Gemm<2, 2, 2, 4, 3, false, false>;   // 128 x 256
-using RowsMany = Gemm<4, 2, 2, 4, 2, false, false>;  // 256 x 256
+// Tiles of the logits (n along the vocabulary x m along the rows), and what a workgroup's step of one takes beside how
+// many run at a time: measured at hidden 2,048, one round of each, in us: 46-50, 31-35, 21-25, 17-20 and 14.5-17.
+using Logits256 = Gemm<4, 2, 2, 4, 2, false, false>;  // 256 x 256
+using Logits128x256 = Gemm<2, 2, 2, 4, 3, false, false>;
+using Logits128 = Gemm<1, 4, 2, 2, 4, false, false>;
+using Logits64 = Gemm<1, 2, 2, 1, 4, false, false>;
+using Logits64x32 = Gemm<1, 2, 1, 1, 4, false, false>;
 // (n along hidden)
 using Dx32 = Gemm<1, 4, 1, 1, 4, true, false>;       // 128 x 32
 using Dx64 = Gemm<1, 4, 2, 1, 3, true, false>;       // 128 x 64
@@ -351,25 +360,48 @@ using Dx128 = Gemm<1, 4, 2, 2, 4, true, false>;      // 128 x 128
 using Dx256 = Gemm<2, 2, 2, 4, 3, true, false>;      // 128 x 256
 using DxMany = Gemm<4, 2, 2, 4, 2, true, false>;     // 256 x 256
 // (n along hidden, m along the vocabulary)
-using Dw = Gemm<4, 2, 2, 4, 2, true, true>;          // 256 x 256
+using Dw256 = Gemm<4, 2, 2, 4, 2, true, true>;       // 256 x 256
+using Dw128 = Gemm<1, 4, 2, 2, 4, true, true>;       // 128 x 128
 
 uint32_t tiles_of(uint64_t n, uint32_t per) { return (uint32_t)((n + per - 1) / per); }
 uint32_t grid_of(uint32_t tiles) { return (tiles + 7) / 8 * 8; }
 
+// The rounds of workgroups that tiles of a kind take, times a round's duration in 1/26 of the largest tiles'.
 template <typename G>
-uint32_t slots_of(uint32_t vocab) { return tiles_of(vocab, G::BN); }
+uint64_t cost_of(uint64_t n, uint64_t m, uint32_t per_cu, uint32_t duration)
+{
+    const uint64_t tiles = (n + G::BN - 1) / G::BN * ((m + G::BM - 1) / G::BM), at_once = per_cu * rl_cu_count();
+    return (tiles + at_once - 1) / at_once * duration;
+}
+
+// Which tiles the logits of so many rows and entries take: those with the fewest rounds for their duration, the largest
+// of them. (At hidden 2,048, in us, the choice and the next best: 100 rows x 16,000 entries 20.7, 23.1; x 32,000 35,
+// 36; 300 x 9,000 26.5, 35; 500 x 16,000 42.8, 52; 1,000 x 4,500 37, 49.)
+int logits_kind(uint32_t rows, uint32_t vocab)
+{
+    const uint64_t cost[5] = {cost_of<Logits256>(vocab, rows, 1, 26), cost_of<Logits128x256>(vocab, rows, 1, 17),
+                              cost_of<Logits128>(vocab, rows, 1, 11), cost_of<Logits64>(vocab, rows, 2, 8),
+                              cost_of<Logits64x32>(vocab, rows, 3, 6)};
+    return (int)(std::min_element(cost, cost + 5) - cost);
+}
 
 uint32_t slots_of(uint32_t rows, uint32_t vocab)
 {
-    return rows <= 32    ? slots_of<Rows32>(vocab)
-           : rows <= 64  ? slots_of<Rows64>(vocab)
-           : rows <= 128 ? slots_of<Rows128>(vocab)
-           : rows <= 256 ? slots_of<Rows256>(vocab)
-                         : slots_of<RowsMany>(vocab);
+    const uint32_t wide[5] = {Logits256::BN, Logits128x256::BN, Logits128::BN, Logits64::BN, Logits64x32::BN};
+    return tiles_of(vocab, wide[logits_kind(rows, vocab)]);
+}
+
+// At least as many statistics as any call up to these rows and entries has: with the largest tiles their own; smaller
+// ones are taken only where they are no slower, so they have at most 26 / duration times the largest's rounds, of all
+// workgroups at a time: up to 430 rows' statistics for each compute unit (the 64 x 64 and 64 x 32 tiles).
+uint64_t most_statistics(uint32_t rows, uint32_t vocab)
+{
+    const uint64_t rounds = cost_of<Logits256>(vocab, rows, 1, 1);
+    return std::max<uint64_t>((uint64_t)tiles_of(vocab, 256) * rows, 430ull * rl_cu_count() * rounds);
 }
 
 template <typename G, bool ROT>
-int launch_stats(LogitParams p)
+int launch_stats(LogitParams &p)
 {
     p.m_tiles = tiles_of(p.rows, G::BM);
     p.n_tiles = tiles_of(p.w.rows, G::BN);
@@ -379,7 +411,7 @@ int launch_stats(LogitParams p)
 }
 
 template <typename G, bool ROT>
-int launch_delta(LogitParams p)
+int launch_delta(LogitParams &p)
 {
     p.m_tiles = tiles_of(p.rows, G::BM);
     p.n_tiles = tiles_of(p.w.rows, G::BN);
@@ -388,12 +420,34 @@ int launch_delta(LogitParams p)
     return rl_check_launch("token_delta_kernel launch");
 }
 
+int launch_stats(LogitParams &p)
+{
+    switch (logits_kind(p.rows, p.w.rows)) {
+    case 0: return launch_stats<Logits256, false>(p);
+    case 1: return launch_stats<Logits128x256, true>(p);
+    case 2: return launch_stats<Logits128, true>(p);
+    case 3: return launch_stats<Logits64, true>(p);
+    default: return launch_stats<Logits64x32, true>(p);
+    }
+}
+
+int launch_delta(LogitParams &p)
+{
+    switch (logits_kind(p.rows, p.w.rows)) {
+    case 0: return launch_delta<Logits256, false>(p);
+    case 1: return launch_delta<Logits128x256, true>(p);
+    case 2: return launch_delta<Logits128, true>(p);
+    case 3: return launch_delta<Logits64, true>(p);
+    default: return launch_delta<Logits64x32, true>(p);
+    }
+}
+
 template <typename G>
 int launch_dx(DxParams p)
 {
     p.m_tiles = tiles_of(p.rows, G::BM);
     p.n_tiles = tiles_of(p.hidden, G::BN);
-    hipLaunchKernelGGL(token_dx_kernel<G>, dim3(grid_of(p.m_tiles * p.n_tiles), p.split), dim3(G::WAVES * 64), 0,
+    hipLaunchKernelGGL(token_dx_kernel<G>, dim3(grid_of(p.m_tiles * p.n_tiles * p.split)), dim3(G::WAVES * 64), 0,
                        rl_stream(), p);
     return rl_check_launch("token_dx_kernel launch");
 }
@@ -536,9 +590,7 @@ extern "C" size_t rl_hip_token_logprob_workspace(const rl_token_logprob_args_t *
 {
     if (validate(a, "rl_hip_token_logprob_workspace") || rl_require_open("rl_hip_token_logprob_workspace"))
         return 0;
-    // (few rows have the smallest tiles)
-    return up256((uint64_t)slots_of<Rows32>(a->vocab) * std::min(a->rows, 256u) * 8) +
-           up256((uint64_t)slots_of<RowsMany>(a->vocab) * a->rows * 8) + up256(a->rows * 4ull);
+    return up256(8 * most_statistics(a->rows, a->vocab)) + up256(a->rows * 4ull);
 }
 
 extern "C" int rl_hip_token_logprob(const rl_token_logprob_args_t *a)
@@ -559,11 +611,7 @@ extern "C" int rl_hip_token_logprob(const rl_token_logprob_args_t *a)
     p.vocab = a->vocab;
     p.part = (rl_f32x2 *)a->workspace;
     p.hit = (float *)((uint8_t *)a->workspace + part);
-    if (a->rows <= 32    ? launch_stats<Rows32, true>(p)
-        : a->rows <= 64  ? launch_stats<Rows64, true>(p)
-        : a->rows <= 128 ? launch_stats<Rows128, true>(p)
-        : a->rows <= 256 ? launch_stats<Rows256, true>(p)
-                         : launch_stats<RowsMany, false>(p))
+    if (launch_stats(p))
         return -1;
     if (slots > 128)
         hipLaunchKernelGGL(token_logprob_kernel<4>, dim3(tiles_of(a->rows, 4)), dim3(256), 0, rl_stream(), p.part, p.hit,
@@ -621,11 +669,7 @@ extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
         const uint16_t *w = (const uint16_t *)a->w + (uint64_t)v0 * a->w_stride;
         p.w = GemmOperand{w, a->w_stride, n, a->hidden};
         p.v0 = v0;
-        if (a->rows <= 32    ? launch_delta<Rows32, true>(p)
-            : a->rows <= 64  ? launch_delta<Rows64, true>(p)
-            : a->rows <= 128 ? launch_delta<Rows128, true>(p)
-            : a->rows <= 256 ? launch_delta<Rows256, true>(p)
-                             : launch_delta<RowsMany, false>(p))
+        if (launch_delta(p))
             return -1;
         if (a->dx) {
             dx.w = GemmOperand{w, a->w_stride, a->hidden, n};
@@ -652,12 +696,14 @@ extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
             // Few rows: little but dw itself moves (200 rows: 326 us for both gradients and the forward pass against
             // 342). With many, the operands that the caches lose cost more (4,096 rows: 3,590 against 3,512).
             dw.past = a->rows <= 512;
-            if (launch_dw<Dw>(dw))
+            // (as for the logits; at 200 rows x 32,000 x 4,096 256 x 256 tiles take 101 us, 128 x 128 106)
+            if (cost_of<Dw128>(dw.hidden, n, 1, 11) < cost_of<Dw256>(dw.hidden, n, 1, 26) ? launch_dw<Dw128>(dw)
+                                                                                         : launch_dw<Dw256>(dw))
                 return -1;
         }
     }
     if (a->dx && !pl.direct) {
-        hipLaunchKernelGGL(token_dx_sum_kernel, dim3(std::min(a->rows, 65535u)), dim3(256), 0, rl_stream(), dx);
+        hipLaunchKernelGGL(token_dx_sum_kernel, dim3(std::min(a->rows * tiles_of(a->hidden, 1024), 1u << 16)), dim3(256), 0, rl_stream(), dx);
         if (rl_check_launch("token_dx_sum_kernel launch"))
             return -1;
     }

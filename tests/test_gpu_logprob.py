@@ -143,6 +143,14 @@ def test_hidden(rl, gpu, hidden, rows):
     c.check(c.run(rl))
 
 
+@pytest.mark.parametrize("rows, vocab", [(500, 32001), (300, 40000), (200, 31990), (490, 16001), (1000, 4500), (120, 30001),
+                                         (300, 8000), (61, 30003), (100, 15000), (70, 2000), (33, 300), (161, 1030)])
+def test_tiles(rl, gpu, rows, vocab):
+    """Every kind of tiles, with several along the rows and the last ones partly filled."""
+    c = Case(rows, rows, vocab, 128, none=0.05)
+    c.check(c.run(rl))
+
+
 @pytest.mark.parametrize("rows, vocab, hidden", [(24, 9000, 512), (130, 9000, 256), (1100, 3000, 512)])
 def test_shares_of_the_vocabulary(rl, gpu, rows, vocab, hidden):
     """dx in shares that are joined; the same bits at every replay."""
