@@ -18,7 +18,16 @@
 //           next one's operands are read from LDS, one read between two matrix
 //           instructions; the barrier of a step stands before its last slice, whose
 //           operands are then in registers, so that the next step's first reads and
-//           the copies into the freed stage run beside matrix instructions too.
+//           the copies into the freed stage run beside matrix instructions too: half of
+//           them in that slice, half in the next (all in one 3 to 5% slower, in three
+//           worse). A wave that has passed the barrier goes first until it has issued
+//           them (2%).
+//  bound    256 x 256 tiles at 2,048 x 128,256 x 4,096: 1,655 us for the statistics,
+//           1,300 TFLOP/s, the chip's power (zeros 1,340 us); there the copies, 64 KiB
+//           a step and compute unit, whose path alone takes 1,410 us (without its
+//           matrix instructions; the matrix instructions alone 1,050). Deeper rings of
+//           32-k steps, prefetching lines into L2 and four waves of 128 x 128 were
+//           slower.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -201,7 +210,10 @@ struct Gemm {
                     wait(s);
                     __builtin_amdgcn_s_barrier();  // step s + 1 is there, and nobody reads step s any more
                     asm volatile("" ::: "memory");
+                    __builtin_amdgcn_s_setprio(1);
                 }
+                if (q == 1)
+                    __builtin_amdgcn_s_setprio(0);
                 constexpr int ALL = TN * TM, READS = TN + TM;
 #pragma unroll
                 for (int i = 0; i < ALL; i++) {
@@ -217,10 +229,17 @@ struct Gemm {
                         else
                             fn[(q + 1) & 1][j - TM] = NT::read(q < 3 ? ns : ns1, nat, j - TM, (q + 1) & 3);
                     }
+                    // (the copies in two parts: all of them behind the barrier are a burst that the matrix
+                    // instructions wait behind)
+                    constexpr int HALF = OPS / 2;
                     if (q == 3 && more)
 #pragma unroll
-                        for (int j = i * OPS / ALL; j < (i + 1) * OPS / ALL; j++)
+                        for (int j = i * HALF / ALL; j < (i + 1) * HALF / ALL; j++)
                             copy(s + NS, j);
+                    if (q == 0 && s > 0 && s - 1 + NS < steps)
+#pragma unroll
+                        for (int j = HALF + i * (OPS - HALF) / ALL; j < HALF + (i + 1) * (OPS - HALF) / ALL; j++)
+                            copy(s - 1 + NS, j);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
