@@ -357,7 +357,6 @@ using Logits64x32 = Gemm<1, 2, 1, 1, 4, false, false>;
 using Dx32 = Gemm<1, 4, 1, 1, 4, true, false>;       // 128 x 32
 using Dx64 = Gemm<1, 4, 2, 1, 3, true, false>;       // 128 x 64
 using Dx128 = Gemm<1, 4, 2, 2, 4, true, false>;      // 128 x 128
-using Dx256 = Gemm<2, 2, 2, 4, 3, true, false>;      // 128 x 256
 using DxMany = Gemm<4, 2, 2, 4, 2, true, false>;     // 256 x 256
 // (n along hidden, m along the vocabulary)
 using Dw256 = Gemm<4, 2, 2, 4, 2, true, true>;       // 256 x 256
@@ -494,8 +493,6 @@ GradPlan plan_of(uint32_t rows, uint32_t vocab, uint32_t hidden)
         dx_shape<Dx64>(rows, hidden, 2, tiles, at_once);
     else if (rows <= 128)
         dx_shape<Dx128>(rows, hidden, 1, tiles, at_once);
-    else if (rows <= 256)
-        dx_shape<Dx256>(rows, hidden, 1, tiles, at_once);
     else
         dx_shape<DxMany>(rows, hidden, 1, tiles, at_once);
     // shares of eight steps at least, of the last piece too
@@ -680,7 +677,6 @@ extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
             if (a->rows <= 32    ? launch_dx<Dx32>(dx)
                 : a->rows <= 64  ? launch_dx<Dx64>(dx)
                 : a->rows <= 128 ? launch_dx<Dx128>(dx)
-                : a->rows <= 256 ? launch_dx<Dx256>(dx)
                                  : launch_dx<DxMany>(dx))
                 return -1;
         }
