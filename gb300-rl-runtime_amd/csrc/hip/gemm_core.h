@@ -121,9 +121,9 @@ struct GemmTile {
     static __device__ __forceinline__ s16x8 read(RL_LDS const uint8_t *stage, const uint32_t (&at)[N], int b, int s)
     {
         if constexpr (KM) {
-            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((RL_LDS s16x4 *)(stage + at[b] + 16 * s * (ROWS * 2)));
-            const s16x4 y =
-                __builtin_amdgcn_ds_read_tr16_b64_v4i16((RL_LDS s16x4 *)(stage + at[b] + (16 * s + 4) * (ROWS * 2)));
+            RL_LDS const uint8_t *from = stage + at[b] + 16 * s * (ROWS * 2);
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((RL_LDS s16x4 *)from);
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((RL_LDS s16x4 *)(from + 4 * (ROWS * 2)));
             return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
         } else {
             return *(RL_LDS const s16x8 *)(stage + at[s] + b * 4096);

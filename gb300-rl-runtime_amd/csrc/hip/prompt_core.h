@@ -324,7 +324,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prompt_kernel(PromptParams p)
     // The row of key or value j (below lk), for what is read from memory once more.
     auto row_of = [&](int plane, uint32_t j) {
         if constexpr (PAGED)
-            return plane_of(x.lost ? 0xFFFFFFFFu : table[j >> p.tpb_shift], plane, j & (p.tpb - 16u)) + (j & 15u) * (uint32_t)D;
+            return plane_of(x.lost ? 0xFFFFFFFFu : table[j >> p.tpb_shift], plane, j & (p.tpb - 16u)) +
+                   (j & 15u) * (uint32_t)D;
         else
             return plane ? vbase + (uint64_t)j * p.v_stride : kbase + (uint64_t)j * p.k_stride;
     };

@@ -75,7 +75,8 @@ __device__ __forceinline__ void turn_of(double pos, double f, float &sine, float
     const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, sum);
     const float y = (float)((quarters - (sum - kRound)) * kQuarter), z = y * y;
     const float s = y + y * z * fmaf(z, fmaf(z, fmaf(z, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6);
-    const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24), -0.5f), 1.f);
+    const float c4 = fmaf(z, fmaf(z, fmaf(z, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24);
+    const float c = fmaf(z, fmaf(z, c4, -0.5f), 1.f);
     const float a = n & 1 ? c : s, b = n & 1 ? s : c;
     sine = n & 2 ? -a : a;
     cosine = (n + 1) & 2 ? -b : b;

@@ -10,8 +10,10 @@
 //            the logits of the piece again, from them D, then its shares of dx and
 //            its rows of dw, both products of D. dx is summed in fp32 over pieces,
 //            and over shares of a piece's vocabulary where its tiles are few.
-//            D's rounding, up to 2^-9 of each element, is of the order of the
-//            outputs' own.
+//            D's rounding, up to 2^-8 of each element, is of the order of the
+//            outputs' own. What it takes from D at a row's target, where D is
+//            largest, is put back in fp32 into dx, and up to 128 rows into dw by a
+//            second part of D.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -58,9 +60,10 @@ struct LogitParams {
     float *hit;              // [rows]: the target's logit
     // gradient
     const float *lse, *grad;
-    uint16_t *d;             // [rows_pad][pitch]
-    uint32_t rows_pad;
+    uint16_t *d;             // [rows_pad][pitch], and behind it what rounding left of it, if `parts` is 2
+    uint32_t rows_pad, parts;
     uint64_t pitch;
+    float *rest;             // [rows]: what rounding left of D at the row's target
 };
 
 template <typename G, bool ROT>
@@ -201,28 +204,41 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_delta_kernel(LogitParams 
                 const float e = __builtin_amdgcn_exp2f((acc[a][b][r] * p.scale - lse) * kLog2e);
                 const float x = g * ((n == at ? 1.f : 0.f) - e);
                 acc[a][b][r] = !has || (!whole && p.v0 + n0 + n >= p.vocab) ? 0.f : x;
+                if (n == at)
+                    p.rest[row] = x - from16<0>(to16<0>(x));
             }
     }
-    uint16_t *d = p.d + nt * G::BN;
-    __syncthreads();  // (nobody reads operands any more)
-    G::template each<false>(acc, smem, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
-        if (m0 + m < p.rows_pad)
-            *(rl_u32x4 *)(d + (uint64_t)(m0 + m) * p.pitch + n) = w;
-        if (G::BM == 32 && m0 + 32 >= p.rows && m0 + 32 < p.rows_pad)  // (rows_pad is a multiple of 64)
-            *(rl_u32x4 *)(d + (uint64_t)(m0 + m + 32) * p.pitch + n) = rl_u32x4{0, 0, 0, 0};
-    });
+    for (uint32_t part = 0; part < p.parts; part++) {
+        if (part)
+#pragma unroll
+            for (int b = 0; b < G::TM; b++)
+#pragma unroll
+                for (int a = 0; a < G::TN; a++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        acc[a][b][r] -= from16<0>(to16<0>(acc[a][b][r]));
+        uint16_t *d = p.d + (uint64_t)part * p.rows_pad * p.pitch + nt * G::BN;
+        __syncthreads();  // (nobody reads operands any more)
+        G::template each<false>(acc, smem, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
+            if (m0 + m < p.rows_pad)
+                *(rl_u32x4 *)(d + (uint64_t)(m0 + m) * p.pitch + n) = w;
+            if (G::BM == 32 && m0 + 32 >= p.rows && m0 + 32 < p.rows_pad)  // (rows_pad is a multiple of 64)
+                *(rl_u32x4 *)(d + (uint64_t)(m0 + m + 32) * p.pitch + n) = rl_u32x4{0, 0, 0, 0};
+        });
+    }
 }
 
-// x with zeros for the rows without a target and those up to rows_pad, which D's zeros alone would not keep out where they
-// are no numbers. A workgroup copies a row at a time.
+// x with zeros for the rows without a target and those up to rows_pad, which D's zeros alone would not keep out where
+// they are no numbers; `parts` times one behind the other. A workgroup copies a row at a time.
 __global__ __launch_bounds__(256) void token_rows_kernel(const uint16_t *x, uint64_t ld, const uint32_t *targets,
-                                                         uint32_t rows, uint32_t rows_pad, uint32_t vocab,
-                                                         uint32_t hidden, uint16_t *out)
+                                                         uint32_t rows, uint32_t rows_pad, uint32_t parts,
+                                                         uint32_t vocab, uint32_t hidden, uint16_t *out)
 {
-    for (uint32_t row = blockIdx.x; row < rows_pad; row += gridDim.x) {
+    for (uint32_t i = blockIdx.x; i < parts * rows_pad; i += gridDim.x) {
+        const uint32_t row = i < rows_pad ? i : i - rows_pad;
         const bool has = row < rows && targets[row] < vocab;
         for (uint32_t c = threadIdx.x; c < hidden / 8; c += 256)
-            *(rl_u32x4 *)(out + (uint64_t)row * hidden + c * 8) =
+            *(rl_u32x4 *)(out + (uint64_t)i * hidden + c * 8) =
                 has ? *(const rl_u32x4 *)(x + row * ld + c * 8) : rl_u32x4{0, 0, 0, 0};
     }
 }
@@ -236,7 +252,19 @@ struct DxParams {
     float *part;      // [split][rows][hidden], or NULL: to dx
     uint16_t *dx;
     uint64_t dx_ld;
+    const uint16_t *w_all;  // the projection, for the targets' rows
+    uint64_t w_ld;
+    const float *rest;
 };
+
+// Four elements from c on of what rounding D at the target took from row `row` of dx (which has a target): there D is
+// largest, and its rounding alone would be up to 2^-8 of the row.
+__device__ __forceinline__ rl_f32x4 target_rest(const DxParams &p, uint32_t row, uint32_t c)
+{
+    const rl_u32x2 w = *(const rl_u32x2 *)(p.w_all + p.targets[row] * p.w_ld + c);
+    const float f = p.rest[row];
+    return rl_f32x4{f * rl_bf16_lo(w[0]), f * rl_bf16_hi(w[0]), f * rl_bf16_lo(w[1]), f * rl_bf16_hi(w[1])};
+}
 
 template <typename G>
 __global__ __launch_bounds__(G::WAVES * 64) void token_dx_kernel(DxParams p)
@@ -271,6 +299,25 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_dx_kernel(DxParams p)
         });
         return;
     }
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int b = 0; b < G::TM; b++) {
+        const uint32_t row = m0 + (wave / G::WN * G::TM + b) * 32 + (lane & 31);
+        if (row >= p.rows || p.targets[row] >= p.vocab)
+            continue;
+#pragma unroll
+        for (int a = 0; a < G::TN; a++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const uint32_t n = n0 + (wave % G::WN * G::TN + a) * 32 + 8 * c + 4 * (lane >> 5);
+                if (n < p.hidden) {
+                    const rl_f32x4 x = target_rest(p, row, n);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        acc[a][b][4 * c + e] += x[e];
+                }
+            }
+    }
     G::template each<false>(acc, smem, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
         if (m0 + m < p.rows && n0 + n < p.hidden) {
             if (p.targets[m0 + m] >= p.vocab)
@@ -302,10 +349,15 @@ __global__ __launch_bounds__(256) void token_dx_sum_kernel(DxParams p)
                     for (int e = 0; e < 4; e++)
                         x[e] += y[k][e];
         }
-        rl_u32x2 w = {(uint32_t)to16<0>(x[0]) | (uint32_t)to16<0>(x[1]) << 16,
-                      (uint32_t)to16<0>(x[2]) | (uint32_t)to16<0>(x[3]) << 16};
-        if (p.targets[row] >= p.vocab)
-            w = rl_u32x2{0, 0};
+        rl_u32x2 w = {0, 0};
+        if (p.targets[row] < p.vocab) {
+            const rl_f32x4 y = target_rest(p, row, c);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                x[e] += y[e];
+            w = rl_u32x2{(uint32_t)to16<0>(x[0]) | (uint32_t)to16<0>(x[1]) << 16,
+                         (uint32_t)to16<0>(x[2]) | (uint32_t)to16<0>(x[3]) << 16};
+        }
         *(rl_u32x2 *)(p.dx + row * p.dx_ld + c) = w;
     }
 }
@@ -456,15 +508,17 @@ int launch_dw(DwParams p)
 {
     p.m_tiles = tiles_of(p.entries, G::BM);
     p.n_tiles = tiles_of(p.hidden, G::BN);
-    hipLaunchKernelGGL(token_dw_kernel<G>, dim3(grid_of(p.m_tiles * p.n_tiles)), dim3(G::WAVES * 64), 0, rl_stream(), p);
+    hipLaunchKernelGGL(token_dw_kernel<G>, dim3(grid_of(p.m_tiles * p.n_tiles)), dim3(G::WAVES * 64), 0, rl_stream(),
+                       p);
     return rl_check_launch("token_dw_kernel launch");
 }
 
 struct GradPlan {
     uint32_t rows_pad, width;  // rows of D, and its columns: entries of a piece, a multiple of 256
+    uint32_t parts;            // of D for dw: with few rows also what its rounding left
     uint32_t split;            // shares of a piece's vocabulary for dx
     bool direct;               // dx from the product itself
-    size_t d, x, part;         // bytes of the workspace's parts
+    size_t d, x, rest, part;   // bytes of the workspace's parts
     size_t most;               // the largest workspace of calls up to this one's rows, vocab and hidden
 };
 
@@ -485,7 +539,13 @@ GradPlan plan_of(uint32_t rows, uint32_t vocab, uint32_t hidden)
     GradPlan pl;
     pl.rows_pad = tiles_of(rows, 64) * 64;
     const uint32_t all = tiles_of(vocab, 256) * 256;
-    pl.width = std::min(all, std::max<uint32_t>(1024, (uint32_t)(kDeltaElements / pl.rows_pad) / 256 * 256));
+    // With few rows a single element of D can be most of a row of dw, and its rounding, up to 2^-8, that row's error;
+    // dw itself is what moves then, and twice the products cost little (forward and gradients of 24 rows x 32,000 x
+    // 4,096 244 us against 232, of 120 292 against 265; of 200 404 against 346: there, as with all more, the
+    // roundings of many rows make dw's error 1.4 times that of its own rounding).
+    pl.parts = rows <= 128 ? 2 : 1;
+    const uint32_t d_rows = pl.parts * pl.rows_pad;
+    pl.width = std::min(all, std::max<uint32_t>(1024, (uint32_t)(kDeltaElements / d_rows) / 256 * 256));
     uint32_t tiles, at_once;
     if (rows <= 32)
         dx_shape<Dx32>(rows, hidden, 2, tiles, at_once);
@@ -499,19 +559,22 @@ GradPlan plan_of(uint32_t rows, uint32_t vocab, uint32_t hidden)
     const uint32_t last = vocab % pl.width ? vocab % pl.width : std::min(pl.width, vocab);
     pl.split = std::max(1u, std::min(at_once / tiles, last / kGemmK / 8));
     pl.direct = pl.split == 1 && pl.width >= vocab;
-    pl.d = up256((uint64_t)pl.rows_pad * pl.width * 2);
-    pl.x = up256((uint64_t)pl.rows_pad * hidden * 2);
+    pl.d = up256((uint64_t)d_rows * pl.width * 2);
+    pl.x = up256((uint64_t)d_rows * hidden * 2);
+    pl.rest = up256(rows * 4ull);
     pl.part = pl.direct ? 0 : up256((uint64_t)pl.split * rows * hidden * 4);
     // D's bound, and as many sums as there are in all tiles at once, or rows
-    const uint64_t d = std::min<uint64_t>((uint64_t)pl.rows_pad * all, std::max<uint64_t>(kDeltaElements, (uint64_t)pl.rows_pad * 1024));
+    const uint64_t most_rows = std::max(d_rows, std::min(256u, 2 * pl.rows_pad));
+    const uint64_t d = std::min(most_rows * all, std::max(kDeltaElements, most_rows * 1024));
     const uint64_t at_most = (uint64_t)rl_cu_count() * (rows <= 128 ? 128 * 128 : 256 * 256);
-    pl.most = up256(2 * d) + pl.x + up256(4 * std::max<uint64_t>((uint64_t)rows * hidden, at_most));
+    pl.most = up256(2 * d) + up256(most_rows * hidden * 2) + pl.rest +
+              up256(4 * std::max<uint64_t>((uint64_t)rows * hidden, at_most));
     return pl;
 }
 
 // What both calls have to have.
-int validate(const char *who, const void *x, const void *w, const void *targets, uint32_t rows, uint32_t vocab, uint32_t hidden,
-             uint32_t x_stride, uint32_t w_stride, float scale)
+int validate(const char *who, const void *x, const void *w, const void *targets, uint32_t rows, uint32_t vocab,
+             uint32_t hidden, uint32_t x_stride, uint32_t w_stride, float scale)
 {
     if (!x || !w || !targets) {
         rl_set_error("%s: NULL argument", who);
@@ -632,13 +695,14 @@ extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
     if (validate(a, who) || rl_require_open(who))
         return -1;
     const GradPlan pl = plan_of(a->rows, a->vocab, a->hidden);
-    if (short_workspace(who, a->workspace, a->workspace_bytes, pl.d + pl.x + pl.part))
+    if (short_workspace(who, a->workspace, a->workspace_bytes, pl.d + pl.x + pl.rest + pl.part))
         return -1;
     uint16_t *d = (uint16_t *)a->workspace, *x = (uint16_t *)((uint8_t *)d + pl.d);
-    float *part = (float *)((uint8_t *)x + pl.x);
+    float *rest = (float *)((uint8_t *)x + pl.x), *part = (float *)((uint8_t *)rest + pl.rest);
     if (a->dw) {
-        hipLaunchKernelGGL(token_rows_kernel, dim3(std::min(pl.rows_pad, 65535u)), dim3(256), 0, rl_stream(),
-                           (const uint16_t *)a->x, a->x_stride, a->targets, a->rows, pl.rows_pad, a->vocab, a->hidden, x);
+        hipLaunchKernelGGL(token_rows_kernel, dim3(std::min(pl.parts * pl.rows_pad, 65535u)), dim3(256), 0, rl_stream(),
+                           (const uint16_t *)a->x, a->x_stride, a->targets, a->rows, pl.rows_pad, pl.parts, a->vocab,
+                           a->hidden, x);
         if (rl_check_launch("token_rows_kernel launch"))
             return -1;
     }
@@ -652,7 +716,9 @@ extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
     p.grad = a->grad_logprob;
     p.d = d;
     p.rows_pad = pl.rows_pad;
+    p.parts = a->dw ? pl.parts : 1;
     p.pitch = pl.width;
+    p.rest = rest;
     DxParams dx = {};
     dx.targets = a->targets;
     dx.rows = a->rows;
@@ -661,6 +727,9 @@ extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
     dx.part = pl.direct ? nullptr : part;
     dx.dx = (uint16_t *)a->dx;
     dx.dx_ld = a->dx_stride;
+    dx.w_all = (const uint16_t *)a->w;
+    dx.w_ld = a->w_stride;
+    dx.rest = rest;
     for (uint32_t v0 = 0; v0 < a->vocab; v0 += pl.width) {
         const uint32_t n = std::min(pl.width, a->vocab - v0);
         const uint16_t *w = (const uint16_t *)a->w + (uint64_t)v0 * a->w_stride;
@@ -682,11 +751,11 @@ extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
         }
         if (a->dw) {
             DwParams dw;
-            dw.x = GemmOperand{x, a->hidden, a->hidden, pl.rows_pad};
-            dw.d = GemmOperand{d, pl.width, pl.width, pl.rows_pad};
+            dw.x = GemmOperand{x, a->hidden, a->hidden, pl.parts * pl.rows_pad};
+            dw.d = GemmOperand{d, pl.width, pl.width, pl.parts * pl.rows_pad};
             dw.entries = n;
             dw.hidden = a->hidden;
-            dw.steps = pl.rows_pad / kGemmK;
+            dw.steps = pl.parts * pl.rows_pad / kGemmK;
             dw.dw = (uint16_t *)a->dw + (uint64_t)v0 * a->dw_stride;
             dw.dw_ld = a->dw_stride;
             // Few rows: little but dw itself moves (200 rows: 326 us for both gradients and the forward pass against
@@ -699,7 +768,8 @@ extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
         }
     }
     if (a->dx && !pl.direct) {
-        hipLaunchKernelGGL(token_dx_sum_kernel, dim3(std::min(a->rows * tiles_of(a->hidden, 1024), 1u << 16)), dim3(256), 0, rl_stream(), dx);
+        hipLaunchKernelGGL(token_dx_sum_kernel, dim3(std::min(a->rows * tiles_of(a->hidden, 1024), 1u << 16)), dim3(256),
+                           0, rl_stream(), dx);
         if (rl_check_launch("token_dx_sum_kernel launch"))
             return -1;
     }

@@ -71,14 +71,16 @@ class Case:
             b.close()
         return out
 
-    def check(self, out, dx=True, dw=True):
+    def check(self, out, dx=True, dw=True, targets_whole=False):
         """Bounds. A logit is an fp32 sum of hidden exact products: off by at most z_off = (hidden + 2) E scale sum |x w|.
         Its exponential's argument (rounded twice, at most 88 where the result counts) and the exponential add 2^-16 of
         it at the most where it is smallest, and less than 2^-20 of the sum; sums of up to 128 in a lane, of two lanes
         and of all tiles' add fewer than 1,200 roundings; the logarithm and the last sum 2^-22 (1 + |lse|). So
         lse_off = z_off + 2^-20 + 1200 E + 2^-22 (1 + |lse|), and a logprob z_off + lse_off + 2 E |logprob|. An element of
         D is off by p (z_off + lse_off + 2^-15) |scale g|, then rounded to bf16: U |D|; the products add fp32 sums of
-        vocab (or rows) terms and one rounding."""
+        vocab (or rows) terms and one rounding. targets_whole: but in dx what rounding takes from D at the target is put
+        back (its product and sum are off by 2 E of it), and with at most 128 rows dw's D is rounded to 16 bits in two
+        parts, U^2 |D| (or 2^-133, below the smallest bf16)."""
         x, w = k8.floats(self.x, "bf16"), k8.floats(self.w, "bf16")
         lp, lse, got_dx, got_dw = out
         has = self.target < self.vocab
@@ -107,12 +109,17 @@ class Case:
             e = np.abs(g_all[r, None]) * p * (z_off + lse_off + 2.0 ** -15)[:, None] + U * 1.01 * np.abs(d)
             if dx:
                 want, mag = d @ w, np.abs(d) @ np.abs(w)
-                tol = e @ np.abs(w) + (self.vocab + 16) * E * mag + U * 1.01 * np.abs(want) + 1e-38
+                e_dx = e.copy()
+                if targets_whole:
+                    e_dx[i, t[r]] -= (U * 1.01 - 2 * E) * np.abs(d[i, t[r]])
+                tol = e_dx @ np.abs(w) + (self.vocab + 16) * E * mag + U * 1.01 * np.abs(want) + 1e-38
                 far = np.abs(k8.floats(got_dx[r, :self.hidden], "bf16") - want)
                 tol[~has[r]] = 0
                 assert (far <= tol).all(), (r0, float((far / (tol + 1e-300)).max()), np.argwhere(~(far <= tol))[:4].tolist())
             if dw:
                 xs = np.where(has[r, None], x[r], 0.0)
+                if targets_whole and self.rows <= 128:
+                    e = e - U * 1.01 * np.abs(d) + 1.01 * U * U * np.abs(d) + 2.0 ** -133
                 ref_dw += d.T @ xs
                 mag_dw += np.abs(d).T @ np.abs(xs)
                 err_dw += e.T @ np.abs(xs)
@@ -141,6 +148,15 @@ def test_vocabularies(rl, gpu, vocab, rows):
 def test_hidden(rl, gpu, hidden, rows):
     c = Case(hidden, rows, 700, hidden, scale=1.25)
     c.check(c.run(rl))
+
+
+@pytest.mark.parametrize("rows, vocab", [(1, 700), (2, 9000), (20, 3000), (33, 500), (60, 30000), (64, 2000), (100, 700),
+                                         (128, 20000), (129, 900), (300, 500), (1000, 300)])
+@pytest.mark.parametrize("lean", [0.0, 5.0])
+def test_what_rounding_takes_at_the_targets(rl, gpu, rows, vocab, lean):
+    """A gradient that is mostly one element of D times a row is not off by that element's rounding to bf16."""
+    c = Case(rows + vocab, rows, vocab, 192, none=0.05 if rows > 2 else 0, lean=lean)
+    c.check(c.run(rl), targets_whole=True)
 
 
 @pytest.mark.parametrize("rows, vocab", [(500, 32001), (300, 40000), (200, 31990), (490, 16001), (1000, 4500), (120, 30001),

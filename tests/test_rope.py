@@ -48,7 +48,8 @@ def rope_args(rl, **kw):
     (dict(kv_heads=0), "kv_heads"), (dict(kv_heads=65536), "kv_heads"), (dict(tokens=3), "tokens"),
     (dict(starts=P, tokens=1 << 31), "tokens"), (dict(arena_base=None, cow_src=P), "cow_src"),
     (dict(arena_bytes=8191), "no block"), (dict(q_stride=4088), "stride"), (dict(q_out_stride=4100), "stride"),
-    (dict(q_stride=4096, q_out_stride=4104), "another stride"), (dict(k_stride=1016), "stride"), (dict(v_stride=1028), "stride"), (dict(k_out=P, k_out_stride=8), "stride"),
+    (dict(q_stride=4096, q_out_stride=4104), "another stride"), (dict(k_stride=1016), "stride"),
+    (dict(v_stride=1028), "stride"), (dict(k_out=P, k_out_stride=8), "stride"),
     (dict(arena_base=P + 8), "aligned"), (dict(q=P + 2), "aligned"), (dict(q_out=P + 8), "aligned"),
     (dict(k_new=P + 4), "aligned"), (dict(v_new=P + 2), "aligned"), (dict(k_out=P + 2), "aligned"),
     (dict(freqs=P + 4), "aligned")])
