@@ -1,5 +1,5 @@
 // attn_chunk.hip - causal attention of chunks of new tokens over the 16-bit paged
-// arena (the kernels are in prompt_core.h).
+// arena (the kernels, what bounds them and what they measure are in prompt_core.h).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

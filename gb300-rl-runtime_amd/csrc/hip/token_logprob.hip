@@ -6,6 +6,9 @@
 //
 //  forward   the product's tiles (gemm_core.h) end in each row's maximum and sum
 //            of exponentials over a wave's columns; a second launch joins them.
+//            Bound by W's stream up to some 100 rows (24 x 32,000 x 4,096 50.6 us, 46 of
+//            them the stream, 5.7 TB/s), by the chip's power with thousands (2,048 x
+//            128,256 x 4,096 1,655-1,755 us, 1,230-1,300 TFLOP/s).
 //  gradient  in pieces of the vocabulary, of which D (bf16) takes up to 256 MiB:
 //            the logits of the piece again, from them D, then its shares of dx and
 //            its rows of dw, both products of D. dx is summed in fp32 over pieces,
@@ -14,6 +17,8 @@
 //            outputs' own. What it takes from D at a row's target, where D is
 //            largest, is put back in fp32 into dx, and up to 128 rows into dw by a
 //            second part of D.
+//            With the forward pass, 4,096 rows x 32,000 x 4,096 take 3,406-3,610 us, 200
+//            rows 332-345.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
