@@ -45,8 +45,7 @@
 //         that the arena does not have reads as keys that are no numbers and values
 //         of 0. Measured, bf16, d128: 2,048 queries of 64 heads behind 30,000 tokens
 //         1,820-1,860 us (1,120-1,145 TFLOP/s of visible pairs), 64 x 1-512 of 32 heads
-//         behind 512 shared ones 236, 64 x 4 behind 512-4,096 120 (5.0 TB/s), 1 x 37
-//         behind 480 12.5.
+//         behind 512 shared ones 236, 64 x 4 behind 512-4,096 120-122 (5.0 TB/s).
 //  softmax online; the maximum a row's weights refer to is raised only when it
 //         is exceeded by more than 2^8, which the fp32 sums and 16-bit weights
 //         hold without loss, so the output is rarely rescaled.

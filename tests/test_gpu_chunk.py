@@ -229,6 +229,57 @@ def test_what_is_not_seen_has_no_part(rl, gpu, d, tpb, dtype):
     assert same[100:, :2].all() and same[100:180, 2:].all() and np.isnan(f[180:, 2:]).all()
 
 
+@pytest.mark.parametrize("d, tpb, qh, kvh, dtype", SHAPES)
+@pytest.mark.parametrize("new", [1, 3, 21])
+def test_few_rows(rl, gpu, d, tpb, qh, kvh, dtype, new):
+    """Few rows, whose keys a workgroup's waves share in runs of 32: every number of runs, whole and not."""
+    ctx = [1, 15, 31, 32, 33, 63, 64, 65, 96, 97, 127, 128, 129, 160, 255, 256, 257, 300, 511, 900]
+    for part in (ctx[:10], ctx[10:]):
+        c = Case(new + d, [min(new, x) for x in part], part, qh, kvh, d, tpb, dtype)
+        out = c.run(rl)
+        c.check(out)
+        assert np.array_equal(c.run(rl, graph=3), out)
+
+
+@pytest.mark.parametrize("d, tpb, dtype", [(128, 16, "bf16"), (64, 32, "bf16"), (128, 32, "fp16"), (64, 16, "fp16")])
+def test_few_rows_what_is_not_seen(rl, gpu, d, tpb, dtype):
+    """As above with few rows; in fp16 also an infinity whose weight 16 bits round to 0."""
+    c = Case(26, [20, 30, 5], [20, 190, 100], 4, 2, d, tpb, dtype)
+    clean = k8.floats(c.run(rl).reshape(c.q.shape), dtype)
+
+    def put(row, head, token, plane, dim, value):
+        c.arena[c.table[row, head, token // tpb], plane, token % tpb, dim] = k8.bits(np.array([value]), dtype)[0]
+
+    put(0, 0, 7, 1, 3, np.nan)
+    put(0, 1, 18, 1, 5, np.inf)
+    put(1, 1, 175, 0, 2, np.nan)           # query 15 of row 1
+    put(1, 0, 40, 1, 9, -np.inf)           # seen by all of row 1
+    f = k8.floats(c.run(rl).reshape(c.q.shape), dtype)
+    tol = 3 * k8.HALF_STEP[dtype] * np.abs(clean) + 4 * k8.HALF_STEP[dtype]
+    same, other = np.abs(f - clean) <= tol, np.arange(d)
+    assert same[:7].all() and np.isnan(f[7:20, :2, 3]).all() and same[7:20, :2][..., other != 3].all()
+    assert same[7:18, 2:].all() and np.isposinf(f[18:20, 2:, 5]).all() and same[18:20, 2:][..., other != 5].all()
+    assert np.isneginf(f[20:50, :2, 9]).all() and same[20:50, :2][..., other != 9].all()
+    assert same[20:35, 2:].all() and np.isnan(f[35:50, 2:]).all() and same[50:].all()
+    # a key of row 2 that all queries weigh with about 2^-40 of the others
+    q = k8.floats(c.q, dtype)
+    q[50:] = np.abs(q[50:])
+    c.q = k8.bits(q, dtype)
+    low = -28.0 * d ** 0.5 / np.abs(q[50:]).sum(-1).min() * np.ones(d)
+    for g in range(2):
+        c.arena[c.table[2, g, 48 // tpb], 0, 48 % tpb] = k8.bits(low, dtype)
+        put(2, g, 48, 1, 11, np.inf)
+    assert np.isposinf(k8.floats(c.run(rl).reshape(c.q.shape), dtype)[50:, :, 11]).all()
+
+
+def test_few_rows_or_many(rl, gpu):
+    """The sizes between which the calls change hands: 256 rows, a workgroup per compute unit, and the keys' times."""
+    for lens, ctx, qh, kvh in (([64, 3], [300, 90], 8, 2), ([65, 3], [300, 90], 8, 2), ([1] * 64, [70] * 64, 4, 4),
+                               ([1] * 65, [70] * 65, 4, 4), ([5], [1200], 8, 2), ([5], [1900], 8, 2)):
+        c = Case(len(lens), lens, ctx, qh, kvh, 64, 16, "bf16")
+        c.check(c.run(rl))
+
+
 def test_equals_a_prompt(rl, gpu):
     """The same tokens as packed rows: rl_hip_attn_prompt's bits."""
     lens, ctx = [70, 12, 200], [70, 300, 333]
