@@ -15,10 +15,10 @@
 //            and over shares of a piece's vocabulary where its tiles are few.
 //            D's rounding, up to 2^-8 of each element, is of the order of the
 //            outputs' own. What it takes from D at a row's target, where D is
-//            largest, is put back in fp32 into dx, and up to 128 rows into dw by a
-//            second part of D.
-//            With the forward pass, 4,096 rows x 32,000 x 4,096 take 3,406-3,610 us, 200
-//            rows 332-345.
+//            largest, is put back in fp32 into dx and dw (up to 128 rows into dw by a
+//            second part of D), whose error is then about that of their own rounding.
+//            With the forward pass, 4,096 rows x 32,000 x 4,096 take 3,420-3,650 us (40 of
+//            them for what is put back), 200 rows 344-348 (14).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -374,7 +374,66 @@ struct DwParams {
     uint16_t *dw;
     uint64_t dw_ld;
     uint32_t past;    // dw is written past the caches
+    const float *rest;        // what rounding left of D at the rows' targets, or NULL: D has a second part
+    const uint32_t *targets;
+    uint32_t rows, v0;        // v0: the piece's first entry
 };
+
+// Puts back what rounding took from D at the targets, for the entries m0 .. of a tile: the first four rows of each (with
+// more, the roundings of many even out), the lowest first.
+template <typename G>
+__device__ __forceinline__ void add_rest(const DwParams &p, uint32_t m0, uint32_t n0, uint32_t *lists,
+                                         typename G::Acc &acc)
+{
+    constexpr uint32_t THREADS = G::WAVES * 64, LONG = 4, NONE = 0xFFFFFFFFu;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (uint32_t i = threadIdx.x; i < LONG * G::BM; i += THREADS)
+        lists[i] = NONE;
+    __syncthreads();
+    // A place of an entry's list keeps the lowest row that it meets and hands the others on to the next, so that the
+    // list is the same whichever row comes first.
+    for (uint32_t r0 = threadIdx.x; r0 < p.rows; r0 += 4 * THREADS) {
+        uint32_t v[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++)
+            v[i] = p.targets[min(r0 + i * THREADS, p.rows - 1)] - p.v0 - m0;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            uint32_t r = r0 + i * THREADS;
+            if (r < p.rows && v[i] < G::BM && m0 + v[i] < p.entries)
+                for (uint32_t k = 0; k < LONG && r != NONE; k++) {
+                    const uint32_t held = atomicMin(lists + k * G::BM + v[i], r);
+                    r = max(held, r);
+                }
+        }
+    }
+    __syncthreads();
+    for (uint32_t k = 0; k < LONG; k++) {
+        const uint32_t *now = lists + k * G::BM;
+#pragma unroll
+        for (int b = 0; b < G::TM; b++) {
+            const uint32_t r = now[(wave / G::WN * G::TM + b) * 32 + (lane & 31)];
+            if (r == NONE)
+                continue;
+            const float f = p.rest[r];
+            const uint16_t *x = p.x.base + r * p.x.ld;
+#pragma unroll
+            for (int a = 0; a < G::TN; a++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const uint32_t n = n0 + (wave % G::WN * G::TN + a) * 32 + 8 * c + 4 * (lane >> 5);
+                    if (n < p.hidden) {
+                        const rl_u32x2 w = *(const rl_u32x2 *)(x + n);
+                        acc[a][b][4 * c] = fmaf(f, rl_bf16_lo(w[0]), acc[a][b][4 * c]);
+                        acc[a][b][4 * c + 1] = fmaf(f, rl_bf16_hi(w[0]), acc[a][b][4 * c + 1]);
+                        acc[a][b][4 * c + 2] = fmaf(f, rl_bf16_lo(w[1]), acc[a][b][4 * c + 2]);
+                        acc[a][b][4 * c + 3] = fmaf(f, rl_bf16_hi(w[1]), acc[a][b][4 * c + 3]);
+                    }
+                }
+        }
+    }
+    __syncthreads();
+}
 
 __device__ __forceinline__ void store16(uint16_t *at, rl_u32x4 w, uint32_t past)
 {
@@ -396,6 +455,8 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_dw_kernel(DwParams p)
     typename G::Acc acc;
     G::run(p.x, p.d, n0, m0, 0, p.steps, 0, smem, acc);
     __syncthreads();  // (nobody reads operands any more)
+    if (p.rest)
+        add_rest<G>(p, m0, n0, (uint32_t *)smem, acc);
     G::template each<false>(acc, smem, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
         if (m0 + m < p.entries && n0 + n < p.hidden)
             store16(p.dw + (m0 + m) * p.dw_ld + n0 + n, w, p.past);
@@ -544,10 +605,8 @@ GradPlan plan_of(uint32_t rows, uint32_t vocab, uint32_t hidden)
     GradPlan pl;
     pl.rows_pad = tiles_of(rows, 64) * 64;
     const uint32_t all = tiles_of(vocab, 256) * 256;
-    // With few rows a single element of D can be most of a row of dw, and its rounding, up to 2^-8, that row's error;
-    // dw itself is what moves then, and twice the products cost little (forward and gradients of 24 rows x 32,000 x
-    // 4,096 244 us against 232, of 120 292 against 265; of 200 404 against 346: there, as with all more, the
-    // roundings of many rows make dw's error 1.4 times that of its own rounding).
+    // With few rows dw itself is what moves, and twice the products cost little: D in two parts (forward and gradients of
+    // 24 rows x 32,000 x 4,096 244 us against 232, of 120 292 against 265; of 200 404 against 346).
     pl.parts = rows <= 128 ? 2 : 1;
     const uint32_t d_rows = pl.parts * pl.rows_pad;
     pl.width = std::min(all, std::max<uint32_t>(1024, (uint32_t)(kDeltaElements / d_rows) / 256 * 256));
@@ -766,6 +825,10 @@ extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
             // Few rows: little but dw itself moves (200 rows: 326 us for both gradients and the forward pass against
             // 342). With many, the operands that the caches lose cost more (4,096 rows: 3,590 against 3,512).
             dw.past = a->rows <= 512;
+            dw.rest = pl.parts == 1 ? rest : nullptr;
+            dw.targets = a->targets;
+            dw.rows = a->rows;
+            dw.v0 = v0;
             // (as for the logits; at 200 rows x 32,000 x 4,096 256 x 256 tiles take 101 us, 128 x 128 106)
             if (cost_of<Dw128>(dw.hidden, n, 1, 11) < cost_of<Dw256>(dw.hidden, n, 1, 26) ? launch_dw<Dw128>(dw)
                                                                                          : launch_dw<Dw256>(dw))

@@ -79,7 +79,8 @@ class Case:
         lse_off = z_off + 2^-20 + 1200 E + 2^-22 (1 + |lse|), and a logprob z_off + lse_off + 2 E |logprob|. An element of
         D is off by p (z_off + lse_off + 2^-15) |scale g|, then rounded to bf16: U |D|; the products add fp32 sums of
         vocab (or rows) terms and one rounding. targets_whole: but in dx what rounding takes from D at the target is put
-        back (its product and sum are off by 2 E of it), and with at most 128 rows dw's D is rounded to 16 bits in two
+        back (its product and sum are off by 2 E of it), in dw too for the first four rows of an entry; with at most 128
+        rows dw's D is rounded to 16 bits in two
         parts, U^2 |D| (or 2^-133, below the smallest bf16)."""
         x, w = k8.floats(self.x, "bf16"), k8.floats(self.w, "bf16")
         lp, lse, got_dx, got_dw = out
@@ -120,6 +121,9 @@ class Case:
                 xs = np.where(has[r, None], x[r], 0.0)
                 if targets_whole and self.rows <= 128:
                     e = e - U * 1.01 * np.abs(d) + 1.01 * U * U * np.abs(d) + 2.0 ** -133
+                elif targets_whole:
+                    first = np.array([(self.target[:r0 + k] == self.target[r0 + k]).sum() < 4 for k in i])
+                    e[i, t[r]] -= np.where(has[r] & first, (U * 1.01 - 2 * E) * np.abs(d[i, t[r]]), 0.0)
                 ref_dw += d.T @ xs
                 mag_dw += np.abs(d).T @ np.abs(xs)
                 err_dw += e.T @ np.abs(xs)
@@ -157,6 +161,17 @@ def test_what_rounding_takes_at_the_targets(rl, gpu, rows, vocab, lean):
     """A gradient that is mostly one element of D times a row is not off by that element's rounding to bf16."""
     c = Case(rows + vocab, rows, vocab, 192, none=0.05 if rows > 2 else 0, lean=lean)
     c.check(c.run(rl), targets_whole=True)
+
+
+@pytest.mark.parametrize("rows, vocab, hidden", [(129, 5000, 192), (200, 300, 64), (700, 2000, 320), (1500, 9, 128)])
+def test_what_rounding_takes_from_many_rows(rl, gpu, rows, vocab, hidden):
+    """The same with more rows than have D in two parts, entries with up to hundreds of rows, and rows that repeat."""
+    c = Case(rows, rows, vocab, hidden, none=0.05, lean=5.0)
+    c.target[rows // 2:rows // 2 + 7] = c.target[0] = 3
+    out = c.run(rl)
+    c.check(out, targets_whole=True)
+    for a, b in zip(out, c.run(rl, graph=2)):
+        assert np.array_equal(a, b)
 
 
 @pytest.mark.parametrize("rows, vocab", [(500, 32001), (300, 40000), (200, 31990), (490, 16001), (1000, 4500), (120, 30001),
