@@ -143,6 +143,9 @@ struct Gemm {
     using Acc = gemm_f32x16[TN][TM];
 
     // The steps kt0 .. kt1 - 1 of the tile at m0, n0 (kt0 < kt1); `rot`: the step to begin with, from which it wraps.
+    // SUMS: eight steps at a time are summed by themselves, so that a sum of 4,096 products is rounded 32 times on its
+    // way and not 256 times.
+    template <bool SUMS = false>
     static __device__ __forceinline__ void run(const GemmOperand &n, const GemmOperand &m, uint32_t n0, uint32_t m0,
                                                uint32_t kt0, uint32_t kt1, uint32_t rot, uint8_t *smem_, Acc &acc)
     {
@@ -192,6 +195,22 @@ struct Gemm {
             rl_wait_vmcnt<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        Acc total;
+        if constexpr (SUMS)
+#pragma unroll
+            for (int a = 0; a < TN; a++)
+#pragma unroll
+                for (int b = 0; b < TM; b++)
+                    total[a][b] = gemm_f32x16{};
+        auto add = [&] {
+#pragma unroll
+            for (int a = 0; a < TN; a++)
+#pragma unroll
+                for (int b = 0; b < TM; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        total[a][b][e] += acc[a][b][e];
+        };
         s16x8 fn[2][TN], fm[2][TM];
 #pragma unroll
         for (int a = 0; a < TN; a++)
@@ -243,6 +262,22 @@ struct Gemm {
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
+            if (SUMS && s % 8 == 7) {
+                add();
+#pragma unroll
+                for (int a = 0; a < TN; a++)
+#pragma unroll
+                    for (int b = 0; b < TM; b++)
+                        acc[a][b] = gemm_f32x16{};
+            }
+        }
+        if constexpr (SUMS) {
+            add();
+#pragma unroll
+            for (int a = 0; a < TN; a++)
+#pragma unroll
+                for (int b = 0; b < TM; b++)
+                    acc[a][b] = total[a][b];
         }
         rl_wait_lgkmcnt0();  // (the reads behind the last step)
     }

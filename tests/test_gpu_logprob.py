@@ -247,6 +247,23 @@ def test_steep_logits(rl, gpu):
     assert out[0].max() > -1e-3 and out[0].min() < -30
 
 
+@pytest.mark.parametrize("rows,vocab", [(1, 4000), (24, 4000), (50, 8000), (100, 16000), (200, 32000)])
+def test_small_products_beside_a_large_one(rl, gpu, rows, vocab):
+    """Every logit is one product of 2^12 and 4,095 of 2^-17. The matrix instruction adds sixteen of these, 2^-13, at a
+    time: to 2^12 in 32 bits they are lost, all 256 of them if the large one comes first. Sums of 512 products are exact
+    unless the large one is among them (512 x 2^-17 lost at most), and each of the eight is added to within half a step
+    of 2^12, 2^-12; so is the logarithm of the entries' number, off by less than 2^-18 with the exponentials' sum."""
+    c = Case(21, rows, vocab, 4096, none=0.0)
+    w = np.full((1, 4096), 2.0 ** -17, np.float32)
+    x = np.ones((rows, 4096), np.float32)
+    w[0, 0] = x[:, 0] = 64.0
+    c.w, c.x = np.ascontiguousarray(np.repeat(k8.bits(w, "bf16"), vocab, 0)), k8.bits(x, "bf16")
+    lp, lse, _, _ = c.run(rl, dx=False, dw=False)
+    ref = 4096 + 4095 * 2.0 ** -17 + np.log(vocab)
+    off = 512 * 2.0 ** -17 + 8 * 2.0 ** -12 + 2.0 ** -12 + 2.0 ** -18
+    assert (np.abs(lse - ref) <= off).all(), float(np.abs(lse - ref).max() / off)
+
+
 def test_strides(rl, gpu):
     c = Case(12, 150, 400, 192)
     plain = c.run(rl)
