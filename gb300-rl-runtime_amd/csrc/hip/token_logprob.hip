@@ -21,7 +21,7 @@
 //            largest, is put back in fp32 into dx and dw (up to 128 rows into dw by a
 //            second part of D), whose error is then about that of their own rounding.
 //            With the forward pass, 4,096 rows x 32,000 x 4,096 take 3,420-3,650 us (40 of
-//            them for what is put back), 200 rows 347-351 (14).
+//            them for what is put back), 200 rows 347-357 (14).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
