@@ -236,6 +236,16 @@ __device__ __forceinline__ void rl_g2lds_16_off(const void *gbase, uint32_t voff
                  : "v"(voff), "s"(base), "s"(lds)
                  : "memory", "m0");
 }
+
+// The same with an address for each lane.
+__device__ __forceinline__ void rl_g2lds_16_at(const void *gsrc, RL_LDS void *lds_base)
+{
+    const uint32_t lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)lds_base);
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                 :
+                 : "v"(gsrc), "s"(lds)
+                 : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 // Waits until at most N vector-memory operations of this wave are

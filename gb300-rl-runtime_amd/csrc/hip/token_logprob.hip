@@ -18,10 +18,12 @@
 //            and over shares of a piece's vocabulary where its tiles are few.
 //            D's rounding, up to 2^-8 of each element, is of the order of the
 //            outputs' own. What it takes from D at a row's target, where D is
-//            largest, is put back in fp32 into dx and dw (up to 128 rows into dw by a
-//            second part of D), whose error is then about that of their own rounding.
-//            With the forward pass, 4,096 rows x 32,000 x 4,096 take 3,420-3,650 us (40 of
-//            them for what is put back), 200 rows 347-357 (14).
+//            largest, is put back into dx and dw, whose error is then about that of
+//            their own rounding: into dw of more than 128 rows by a product of the rows
+//            that have a target in a tile, however many rows an entry has (tokens are
+//            not spread evenly); up to 128 rows by a second part of D.
+//            With the forward pass, 4,096 rows x 32,000 x 4,096 take 3,420-3,650 us,
+//            200 rows 347-357; with all rows of one target 5% and 2% more.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -384,60 +386,108 @@ struct DwParams {
     uint32_t rows, v0;        // v0: the piece's first entry
 };
 
-// Puts back what rounding took from D at the targets, for the entries m0 .. of a tile: the first four rows of each (with
-// more, the roundings of many even out), the lowest first.
+// Puts back what rounding took from D at the targets, for the entries m0 .. of a tile: the product of x with a matrix
+// that has one element in each row with a target here. Such rows are listed in order, so that the sums are the same
+// every time, and taken 64 at a time: their x through LDS as an operand of D's product is, the elements from registers, in
+// two bf16 parts, which hold all of an element's at most 16 bits. An entry may have any number of rows.
 template <typename G>
-__device__ __forceinline__ void add_rest(const DwParams &p, uint32_t m0, uint32_t n0, uint32_t *lists,
+__device__ __forceinline__ void add_rest(const DwParams &p, uint32_t m0, uint32_t n0, uint8_t *smem_,
                                          typename G::Acc &acc)
 {
-    constexpr uint32_t THREADS = G::WAVES * 64, LONG = 4, NONE = 0xFFFFFFFFu;
+    using X = typename G::NT;
+    constexpr uint32_t THREADS = G::WAVES * 64, SPAN = 4 * THREADS, MASKS = SPAN / 64, NONE = 0xFFFFFFFFu;
+    static_assert(MASKS <= 64, "a mask for each lane at the most");
+    static_assert(X::BYTES + SPAN * 4 + (SPAN + 64) * 8 + MASKS * 8 <= G::LDS, "room for the lists");
+    RL_LDS uint8_t *stage = (RL_LDS uint8_t *)smem_;
+    RL_LDS rl_u32x2 *what = (RL_LDS rl_u32x2 *)(stage + X::BYTES);  // entry, both parts
+    RL_LDS uint32_t *rows = (RL_LDS uint32_t *)(what + SPAN + 64);
+    RL_LDS uint64_t *masks = (RL_LDS uint64_t *)(rows + SPAN);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (uint32_t i = threadIdx.x; i < LONG * G::BM; i += THREADS)
-        lists[i] = NONE;
-    __syncthreads();
-    // A place of an entry's list keeps the lowest row that it meets and hands the others on to the next, so that the
-    // list is the same whichever row comes first.
-    for (uint32_t r0 = threadIdx.x; r0 < p.rows; r0 += 4 * THREADS) {
+    const uint32_t wn = wave % G::WN, wm = wave / G::WN, hf = lane >> 5;
+    uint32_t at[G::TN];
+    X::template places<G::TN>(wn * G::TN, (int)lane, at);
+    for (uint32_t r0 = 0; r0 < p.rows; r0 += SPAN) {
         uint32_t v[4];
+        uint64_t has[4];
 #pragma unroll
         for (uint32_t i = 0; i < 4; i++)
-            v[i] = p.targets[min(r0 + i * THREADS, p.rows - 1)] - p.v0 - m0;
+            v[i] = p.targets[min(r0 + i * THREADS + threadIdx.x, p.rows - 1)] - p.v0 - m0;
 #pragma unroll
         for (uint32_t i = 0; i < 4; i++) {
-            uint32_t r = r0 + i * THREADS;
-            if (r < p.rows && v[i] < G::BM && m0 + v[i] < p.entries)
-                for (uint32_t k = 0; k < LONG && r != NONE; k++) {
-                    const uint32_t held = atomicMin(lists + k * G::BM + v[i], r);
-                    r = max(held, r);
-                }
+            const uint32_t r = r0 + i * THREADS + threadIdx.x;
+            v[i] = r < p.rows && v[i] < G::BM && m0 + v[i] < p.entries ? v[i] : NONE;
+            has[i] = __builtin_amdgcn_ballot_w64(v[i] != NONE);
+            if (lane == 0)
+                masks[i * G::WAVES + wave] = has[i];
         }
-    }
-    __syncthreads();
-    for (uint32_t k = 0; k < LONG; k++) {
-        const uint32_t *now = lists + k * G::BM;
+        __syncthreads();
+        uint32_t upto = lane < MASKS ? (uint32_t)__builtin_popcountll(masks[lane]) : 0u;
 #pragma unroll
-        for (int b = 0; b < G::TM; b++) {
-            const uint32_t r = now[(wave / G::WN * G::TM + b) * 32 + (lane & 31)];
-            if (r == NONE)
-                continue;
-            const float f = p.rest[r];
-            const uint16_t *x = p.x.base + r * p.x.ld;
+        for (uint32_t d = 1; d < 64; d *= 2) {
+            const uint32_t before = __shfl_up(upto, d);
+            upto += lane >= d ? before : 0u;
+        }
+        const uint32_t n = rl_readlane(upto, 63);
 #pragma unroll
-            for (int a = 0; a < G::TN; a++)
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t mask = i * G::WAVES + wave, first = mask ? rl_readlane(upto, (int)mask - 1) : 0u;
+            if (v[i] != NONE) {
+                const uint32_t to = first + __builtin_amdgcn_mbcnt_hi((uint32_t)(has[i] >> 32),
+                                                                      __builtin_amdgcn_mbcnt_lo((uint32_t)has[i], 0));
+                const uint32_t r = r0 + i * THREADS + threadIdx.x;
+                const float f = p.rest[r];
+                const uint32_t high = to16<0>(f);
+                rows[to] = r;
+                what[to] = rl_u32x2{v[i], high | (uint32_t)to16<0>(f - from16<0>((uint16_t)high)) << 16};
+            }
+        }
+        if (threadIdx.x < 64)  // (up to a whole step: no row's)
+            what[n + threadIdx.x] = rl_u32x2{NONE, 0u};
+        __syncthreads();
+        for (uint32_t k0 = 0; k0 < n; k0 += 64) {
+            const uint32_t slices = min(4u, (n - k0 + 15) / 16);  // of 16 rows
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const uint32_t n = n0 + (wave % G::WN * G::TN + a) * 32 + 8 * c + 4 * (lane >> 5);
-                    if (n < p.hidden) {
-                        const rl_u32x2 w = *(const rl_u32x2 *)(x + n);
-                        acc[a][b][4 * c] = fmaf(f, rl_bf16_lo(w[0]), acc[a][b][4 * c]);
-                        acc[a][b][4 * c + 1] = fmaf(f, rl_bf16_hi(w[0]), acc[a][b][4 * c + 1]);
-                        acc[a][b][4 * c + 2] = fmaf(f, rl_bf16_lo(w[1]), acc[a][b][4 * c + 2]);
-                        acc[a][b][4 * c + 3] = fmaf(f, rl_bf16_hi(w[1]), acc[a][b][4 * c + 3]);
+            for (uint32_t i = 0; i < X::OPS; i++) {
+                const uint32_t first = (wave * X::OPS + i) * X::PER, k = first + lane / X::NC;
+                if (first >= 16 * slices)
+                    break;
+                // (past the last row it again, beside elements of 0)
+                const uint32_t c = n0 + 8 * ((lane % X::NC) ^ X::swz(k));
+                rl_g2lds_16_at(p.x.base + rows[min(k0 + k, n - 1)] * p.x.ld + min(c, p.hidden - 8),
+                            stage + (wave * X::OPS + i) * 1024);
+            }
+            rl_wait_vmcnt<0>();
+            __syncthreads();
+            for (uint32_t s = 0; s < slices; s++) {
+                RL_LDS const rl_u32x2 *of = what + k0 + 16 * s + 8 * hf;
+                RL_LDS const uint8_t *from = stage + 16 * s * (G::BN * 2);
+                s16x8 fn[G::TN];
+#pragma unroll
+                for (int a = 0; a < G::TN; a++)
+                    fn[a] = X::read(from, at, a, 0);
+#pragma unroll
+                for (int b = 0; b < G::TM; b++) {
+                    const uint32_t m = (wm * G::TM + b) * 32 + (lane & 31);
+                    rl_u32x4 high, low;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const uint32_t x = of[2 * e][0] == m ? of[2 * e][1] : 0u;
+                        const uint32_t y = of[2 * e + 1][0] == m ? of[2 * e + 1][1] : 0u;
+                        high[e] = (x & 0xFFFFu) | y << 16;
+                        low[e] = x >> 16 | (y & 0xFFFF0000u);
+                    }
+#pragma unroll
+                    for (int a = 0; a < G::TN; a++) {
+                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                            __builtin_bit_cast(bf16x8, fn[a]), __builtin_bit_cast(bf16x8, high), acc[a][b], 0, 0, 0);
+                        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                            __builtin_bit_cast(bf16x8, fn[a]), __builtin_bit_cast(bf16x8, low), acc[a][b], 0, 0, 0);
                     }
                 }
+            }
+            __syncthreads();  // (nobody reads this step's rows any more)
         }
     }
-    __syncthreads();
 }
 
 __device__ __forceinline__ void store16(uint16_t *at, rl_u32x4 w, uint32_t past)
@@ -461,7 +511,7 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_dw_kernel(DwParams p)
     G::run(p.x, p.d, n0, m0, 0, p.steps, 0, smem, acc);
     __syncthreads();  // (nobody reads operands any more)
     if (p.rest)
-        add_rest<G>(p, m0, n0, (uint32_t *)smem, acc);
+        add_rest<G>(p, m0, n0, smem, acc);
     G::template each<false>(acc, smem, [&](uint32_t m, uint32_t n, rl_u32x4 w) {
         if (m0 + m < p.entries && n0 + n < p.hidden)
             store16(p.dw + (m0 + m) * p.dw_ld + n0 + n, w, p.past);

@@ -370,8 +370,8 @@ int rl_hip_logits_proj(const rl_logits_proj_args_t *args);
  *   D[r][v] = scale * grad_logprob[r] * (1[v = targets[r]] - exp(z[r][v] - lse[r]))
  *   dx = D w    dw = D^T x
  * in pieces of the vocabulary whose logits are computed again; D is rounded to
- * bf16 (but for what that would take at the targets, with up to four rows of one
- * target), sums are fp32 and each result is rounded once. dx or dw may be NULL.
+ * bf16 (but for what that would take at the targets, which is put back), sums are
+ * fp32 and each result is rounded once. dx or dw may be NULL.
  * Rows without a target have no part in either, whatever they hold, and get
  * zeros in dx. Outputs may not overlap inputs. The same call gives the same bits. */
 typedef struct {
