@@ -53,10 +53,10 @@ __device__ __forceinline__ float pair_sum(float x)
 // Maximum and sum of exponentials of two sets together.
 __device__ __forceinline__ rl_f32x2 join(rl_f32x2 x, rl_f32x2 y)
 {
-    // (a set without a maximum has the sum 0, or none that is a number)
+    // (an equal maximum is no difference: two infinities have none that is a number)
     const float top = fmaxf(x[0], y[0]);
-    return rl_f32x2{top, x[1] * (x[0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((x[0] - top) * kLog2e)) +
-                             y[1] * (y[0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((y[0] - top) * kLog2e))};
+    return rl_f32x2{top, x[1] * (x[0] == top ? 1.f : __builtin_amdgcn_exp2f((x[0] - top) * kLog2e)) +
+                             y[1] * (y[0] == top ? 1.f : __builtin_amdgcn_exp2f((y[0] - top) * kLog2e))};
 }
 
 struct LogitParams {
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_stats_kernel(LogitParams 
                 top = fmaxf(top, z);
             }
         top = pair_max(top);
-        const float ref = top == -INFINITY ? 0.f : top;
+        const float ref = fabsf(top) == INFINITY ? 0.f : top;  // (the exponentials are then 0 and infinity)
 #pragma unroll
         for (int a = 0; a < G::TN; a++)
 #pragma unroll
