@@ -12,7 +12,9 @@
 //         and cosine (to the 10th) are within 2^-24.
 //  bound  the bytes: 64 prompts of 512-1,024 tokens, 32 query and 8 KV heads of d128,
 //         211-226 us (5.3-5.7 TB/s, a copy's rate); one token of 64 rows 3.1-4.0 us, a
-//         launch and the chain position, table entry, store.
+//         launch and the chain position, table entry, store. Copies on write, each a
+//         wave's, add 0.2-0.3 us to 64 rows of 8 KV heads (one token 3.2 to 3.4, 200
+//         tokens 62.8 to 63.1).
 //  split  a lane holds two 16-byte chunks of a head, those that are turned into
 //         each other, of one token; a wave D / 16 lanes for each of its 8 (d128)
 //         or 16 (d64) tokens, and goes through some of their heads, so that

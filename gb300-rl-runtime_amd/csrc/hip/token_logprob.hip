@@ -520,7 +520,8 @@ __global__ __launch_bounds__(G::WAVES * 64) void token_dw_kernel(DwParams p)
 
 // ---- the host's side ----------------------------------------------------------------
 // Tiles of the logits (n along the vocabulary x m along the rows), and what a workgroup's step of one takes beside how
-// many run at a time: measured at hidden 2,048, one round of each, in us: 46-50, 31-35, 21-25, 17-20 and 14.5-17.
+// many run at a time: measured at hidden 2,048, one round of each, in us: 46-50, 31-35, 21-25, 17-20 and 14.5-17, some 4.5
+// of them the launch; the rest are as 26 to 17, 11, 8 and 6.
 using Logits256 = Gemm<4, 2, 2, 4, 2, false, false>;  // 256 x 256
 using Logits128x256 = Gemm<2, 2, 2, 4, 3, false, false>;
 using Logits128 = Gemm<1, 4, 2, 2, 4, false, false>;
@@ -884,7 +885,8 @@ extern "C" int rl_hip_token_logprob_grad(const rl_token_logprob_grad_args_t *a)
             dw.targets = a->targets;
             dw.rows = a->rows;
             dw.v0 = v0;
-            // (as for the logits; at 200 rows x 32,000 x 4,096 256 x 256 tiles take 101 us, 128 x 128 106)
+            // (as for the logits; at 200 rows x 32,000 x 4,096, what rounding took put back, 256 x 256 tiles take 111 us,
+            // 128 x 128 188; at 4,096 rows 923 and 1,534)
             if (cost_of<Dw128>(dw.hidden, n, 1, 11) < cost_of<Dw256>(dw.hidden, n, 1, 26) ? launch_dw<Dw128>(dw)
                                                                                          : launch_dw<Dw256>(dw))
                 return -1;

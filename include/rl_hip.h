@@ -239,7 +239,8 @@ int rl_rope_freqs(double *freqs, uint32_t rot_dim, double theta);
  * query i of Lq sees the keys j <= i + ctx_lens[b] - Lq. One token per row is a
  * decode step; more are a piece of a prompt, or drafted tokens to be checked.
  * Heads, sums and rounding, queries that see no key, values that are no numbers
- * and rows of out that belong to no sequence are as in rl_hip_attn_prompt. A row
+ * and rows of out that belong to no sequence are as in rl_hip_attn_prompt (also for
+ * one token, whose weights rl_hip_attn_decode keeps more bits of). A row
  * whose context exceeds max_ctx gets NaN outputs, and so does every query that
  * sees a key of a block past arena_bytes (which is not read). */
 typedef struct {
