@@ -364,7 +364,7 @@ int rl_hip_logits_proj(const rl_logits_proj_args_t *args);
  *   lse[r] = log sum_v exp z[r][v]    logprob[r] = z[r][targets[r]] - lse[r]
  * without keeping the logits. A row whose target is `vocab` or more (the places
  * behind a rollout's end, say) has logprob 0, its lse all the same.
- * Logits that are infinite count as the formula has them: lse is infinity beside one.
+ * Infinite logits count as the formula has them: one of +infinity makes lse infinity.
  *
  * rl_hip_token_logprob_grad is its gradient: from lse and grad_logprob[r], the
  * derivative of the loss by logprob[r] (for -mean(advantage * logprob): the
